@@ -18,7 +18,7 @@
 //     first ch*cw lanes and broadcast through LDS;
 //   - the inner loop is kept lean because the CU's vector-memory path is the co-limiter (4 tap loads + 1 store of
 //     16 B per lane = 2.78 GB per launch through 64 B/clk/CU; TA busy 75 % in profiles/r01_pmc_crop_*): SGPR-base +
-//     32-bit lane offsets (no 64-bit address arithmetic), packed fp32 lerps, 4 outputs (16 taps) in flight per lane
+//     32-bit lane offsets (no 64-bit address arithmetic), fp32 lerps, 4 outputs (16 taps) in flight per lane
 //     at 4 waves per SIMD.
 //   Rejected after measurement (tools/crop_bench.hip): a (box, 256-B channel chunk) workgroup cuts L2 reads by 32 %
 //   through L1 reuse yet runs 12-20 % slower (more workgroups, same bytes through the vector-memory path); staging the
@@ -103,36 +103,21 @@ __device__ __forceinline__ PixParam pix_param(int p, int H, int W, unsigned pix_
   return prm;
 }
 
-// a - b on the packed-fp32 pipe: v_pk_add_f32 with the neg modifier on b (exactly a - b); the compiler packs fadd/fmul of
-// <4 x float> but splits fsub into four v_sub_f32.
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ float vsub(float a, float b) { return a - b; }
-__device__ __forceinline__ f32x4 vsub(f32x4 a, f32x4 b) {
-  f32x2 lo, hi;
-  const f32x2 alo = a.xy, ahi = a.zw, blo = b.xy, bhi = b.zw;
-  asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(lo) : "v"(alo), "v"(blo));
-  asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(hi) : "v"(ahi), "v"(bhi));
-  f32x4 r;
-  r.xy = lo;
-  r.zw = hi;
-  return r;
-}
-
 // One bilinear sample: three lerps, one rounding per operation.  `base` is wave-uniform and the lane offset 32-bit, so
-// the loads take the SGPR-base + VGPR-offset form (no 64-bit address arithmetic per tap); subtractions go through vsub (packed).
+// the loads take the SGPR-base + VGPR-offset form (no 64-bit address arithmetic per tap).
 template <class vec_t>
 __device__ __forceinline__ vec_t bilerp(const char *__restrict__ base, const PixParam &prm, unsigned cb, float extrap) {
   const vec_t tl = *reinterpret_cast<const vec_t *>(base + (size_t)(prm.off_tl + cb));
   const vec_t tr = *reinterpret_cast<const vec_t *>(base + (size_t)(prm.off_tr + cb));
   const vec_t bl = *reinterpret_cast<const vec_t *>(base + (size_t)(prm.off_bl + cb));
   const vec_t br = *reinterpret_cast<const vec_t *>(base + (size_t)(prm.off_br + cb));
-  vec_t t = vsub(tr, tl);
+  vec_t t = tr - tl;
   t = t * prm.lx;
   const vec_t tp = tl + t;
-  t = vsub(br, bl);
+  t = br - bl;
   t = t * prm.lx;
   const vec_t bt = bl + t;
-  t = vsub(bt, tp);
+  t = bt - tp;
   t = t * prm.ly;
   vec_t v = tp + t;
   if (!prm.valid) v = (vec_t)(extrap);
@@ -562,13 +547,13 @@ __global__ __launch_bounds__(NT) void crop_resize_rowstage_kernel(StageGroups gr
         const unsigned cc = in ? (unsigned)c : 0u;
         // the three lerps of bilerp(), one rounding per operation, taps from LDS
         const f32x4 tl = rows[prm.off_tl + cc], tr = rows[prm.off_tr + cc], bl = rows[prm.off_bl + cc], br = rows[prm.off_br + cc];
-        f32x4 tt = vsub(tr, tl);
+        f32x4 tt = tr - tl;
         tt = tt * prm.lx;
         const f32x4 tp = tl + tt;
-        tt = vsub(br, bl);
+        tt = br - bl;
         tt = tt * prm.lx;
         const f32x4 bt = bl + tt;
-        tt = vsub(bt, tp);
+        tt = bt - tp;
         tt = tt * prm.ly;
         f32x4 val = tp + tt;
         if (!prm.valid) val = (f32x4)(extrap);
@@ -700,8 +685,7 @@ void crop_resize_kernel(
 #ifndef FRCNN_CROP_UNROLL
 #define FRCNN_CROP_UNROLL 4
 #endif
-    // FRCNN_CROP_UNROLL outputs per lane per trip, all their taps issued before the first lerp.  Unrolled by hand (the
-    // packed-subtract asm is convergent, which rules out the compiler's runtime unroll): lanes past the end recompute
+    // FRCNN_CROP_UNROLL outputs per lane per trip, all their taps issued before the first lerp.  Unrolled by hand: lanes past the end recompute
     // the last element (in-bounds loads) and skip the store.
     for (int e0 = tid; e0 < total; e0 += FRCNN_CROP_NT * FRCNN_CROP_UNROLL) {
       vec_t v[FRCNN_CROP_UNROLL];

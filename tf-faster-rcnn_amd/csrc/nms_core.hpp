@@ -128,9 +128,8 @@ __device__ __forceinline__ bool nms_iou_gt_fast(const PBox &i, const PBox &j, co
 }
 
 // The band filter for TWO row boxes (a, b) against one box `me`, all three REGULAR (finite, area in [1e-30, 5e29]: no
-// flags to look at), as packed fp32: the subtractions, products and scalings of the two tests share v_pk_add_f32 /
-// v_pk_mul_f32 (10 VALU instructions per pair instead of 19; only max / min have no packed form), in the union-free form
-// described at IouThr.  a_area2 = (area a, area b).
+// flags to look at), written on pairs, in the union-free form described at IouThr (the library is built without the packed
+// fp32 instructions, so a pair costs two scalar ones).  a_area2 = (area a, area b).
 typedef float v2f __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void nms_iou_gt_fast2(const float4 &me, float me_area, const float4 &a, const float4 &b, v2f ab_area,
                                                  const IouThr &t, bool &yes_a, bool &yes_b, bool &irr) {
