@@ -252,6 +252,64 @@ int frcnn_roi_delta(const float *rois, const float *gt_boxes, const int32_t *gt_
                     float *out_deltas, float *out_labels, void *workspace, size_t workspace_bytes,
                     frcnn_stream_t stream);
 
+/* ---- the detection head: dense products in 8-bit floating point, group normalisation, dropout ---------------------------- */
+/* What stands between RoIPooling and Decoder in the reference's model (models/faster_rcnn.py:320-326: Flatten, two Dense of
+ * 4096 with relu, each followed by Dropout, and the two output Dense layers), as operators.  Element types, scale types and
+ * activations of these entry points: */
+#define FRCNN_F32 0
+#define FRCNN_F16 1
+#define FRCNN_BF16 2
+#define FRCNN_SCALE_F32 0
+#define FRCNN_SCALE_E8M0 1 /* one byte: 2^(byte - 127), 255 = NaN */
+#define FRCNN_ACT_NONE 0
+#define FRCNN_ACT_RELU 1
+#define FRCNN_ACT_SWISH 2 /* z / (1 + exp(-z)) */
+
+/* Rows of x (rows, K; row stride ldx elements) to OCP e4m3 with one scale per block of block_rows (1 or 128) x 128 elements:
+ * scale = max(amax / 448, 2^-126) over the block's finite values, 1 where they are all zero (FRCNN_SCALE_E8M0: the smallest
+ * power of two that is not below amax / 448, 2^-126 at least); q = x / scale rounded to nearest even.  NaN and infinities
+ * become e4m3's NaN.  q (rows, K) has the row stride ldq, a multiple of 16, and starts at a multiple of 16 bytes; of each row
+ * the bytes up to the next multiple of 16 are written (zeros behind K).  Scale (r / block_rows, kb) is written to
+ * scales[(r / block_rows) * scale_row_stride + kb * scale_block_stride] (strides in elements). */
+int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int rows, int K, int block_rows, void *q, int64_t ldq,
+                          void *scales, int scale_type, int64_t scale_row_stride, int64_t scale_block_stride,
+                          frcnn_stream_t stream);
+
+/* y (M, N; row stride ldy) = act(sum over blocks kb of 128 columns of a_scale(m, kb) * b_scale(n / 128, kb) * the block's
+ * dot product of a's row m and b's row n, + bias[n]).  a (M, K) and b (N, K): e4m3, rows 16-byte aligned (row strides in
+ * bytes, multiples of 16; nothing behind a row's K bytes is read); scales as frcnn_quantize_blocks leaves them with
+ * block_rows 1 for a and 128 for b, both of scale_type.  bias (N) fp32 or NULL.  activation: none or relu.  Sums are held in
+ * fp32.  K == 0 gives act(bias).  Limits: K <= 2^22, row strides <= 2^23 bytes, N <= 2^24. */
+size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K);
+int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_scale_row_stride,
+                        int64_t a_scale_block_stride, const void *b, int64_t ldb, const void *b_scales,
+                        int64_t b_scale_row_stride, int64_t b_scale_block_stride, int scale_type, const float *bias,
+                        int activation, int M, int N, int K, void *y, int y_type, int64_t ldy, void *workspace,
+                        size_t workspace_bytes, frcnn_stream_t stream);
+
+/* Group normalisation of a channels-last tensor x (N, S, C) of `type`, C in G groups of neighbouring channels: mean and
+ * variance per image and group over S * (C / G) values, y = act((x - mean) / sqrt(var + epsilon) * gamma + beta).  gamma,
+ * beta (C) fp32.  stats (N, G, 2) fp32 receives mean and 1 / sqrt(var + epsilon) (NULL: not wanted).  S >= 1.  Groups of up
+ * to 512 channels always, of up to 512 * 16 / sizeof(type) where 16 / sizeof(type) divides C / G and all rows are 16-byte
+ * aligned. */
+size_t frcnn_group_norm_workspace_bytes(int type, int64_t N, int64_t S, int C, int G);
+int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int C, int G, const float *gamma, const float *beta,
+                     float epsilon, int activation, void *y, float *stats, void *workspace, size_t workspace_bytes,
+                     frcnn_stream_t stream);
+/* Its gradients: dx of dy's type, dgamma and dbeta (C) fp32, from dy, x and the stats of the forward call.  Summed in a fixed
+ * order: the same inputs give the same bits. */
+size_t frcnn_group_norm_grad_workspace_bytes(int type, int64_t N, int64_t S, int C, int G);
+int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, int64_t S, int C, int G, const float *gamma,
+                          const float *beta, const float *stats, int activation, void *dx, float *dgamma, float *dbeta,
+                          void *workspace, size_t workspace_bytes, frcnn_stream_t stream);
+
+/* y[i] = x[i] / (1 - rate) where word i % 4 of block i / 4 of Philox4x32 with 7 rounds (key: seed; counter: block number,
+ * offset; 64 bits each) is at least round(rate * 2^32), else 0.  0 <= rate < 1.  state: NULL, or a device pointer to
+ * {seed, offset} that replaces the two arguments (a captured graph then draws by what it finds there at each replay).
+ * The gradient is the same call on dy. */
+int frcnn_dropout(const void *x, void *y, int type, int64_t count, double rate, uint64_t seed, uint64_t offset,
+                  const uint64_t *state, frcnn_stream_t stream);
+
 /* ---- host gather ----------------------------------------------------------------------- */
 /* Copy `bytes` bytes from device memory to `dst`, which may be pinned host memory mapped into the device (hipHostMalloc):
  * the "final host gather" of the small per-image outputs in a deployment sharded over GPUs (there is no counterpart in the

@@ -1,0 +1,644 @@
+"""The detection head's operators against their formulas in 64 bits.
+
+Tolerances count roundings: a result of type t is off by at most half a step, eps(t) / 2 of its value, beyond what the fp32
+sums before it are; an fp32 sum of n terms in any order is off by at most n * 2^-24 of the sum of their magnitudes.
+"""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+E8M0 = torch.float8_e8m0fnu
+U = 2.0 ** -24  # half a step of fp32
+
+
+@pytest.fixture(scope="module")
+def head():
+    import tf_faster_rcnn_amd as pkg
+    return pkg.head_utils
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+# ---- quantize_blocks ----------------------------------------------------------------------------------------------------------
+def e4m3_nearest(v):
+    """Nearest e4m3 to each |v| <= 448 in 64 bits, ties to even; NaN stays."""
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))) - 3)
+    return torch.round(v / step) * step
+
+
+def quantized(x, block_rows, scale_dtype):
+    """(values, scales) by the definition.  The scale and the quotient are fp32 operations of the definition, each correctly
+    rounded: 64-bit division of fp32 numbers rounded to fp32 is the correctly rounded fp32 quotient (53 >= 2 * 24 + 2)."""
+    rows, inner = x.shape
+    up, across = -(-rows // block_rows), -(-inner // 128)
+    v = torch.zeros((up * block_rows, across * 128), dtype=torch.float64, device=x.device)
+    v[:rows, :inner] = x.double()
+    v = v.view(up, block_rows, across, 128)
+    amax = torch.where(torch.isfinite(v), v.abs(), 0.0).amax((1, 3))
+    if scale_dtype == F32:
+        s = (amax / 448).float().double().clamp_min(2.0 ** -126)
+    else:
+        f, e = torch.frexp(amax)
+        e = (e - 9 + (f > 0.875).int()).clamp_min(-126)
+        s = torch.from_numpy(np.ldexp(1.0, e.cpu().numpy())).cuda()  # torch.ldexp goes through an fp32 power
+    s = torch.where(amax > 0, s, 1.0)
+    q = (v / s[:, None, :, None]).float().double()
+    q = torch.where(torch.isfinite(v), e4m3_nearest(q), float("nan"))
+    return q.view(up * block_rows, across * 128)[:rows, :inner], s
+
+
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,inner", [(1, 1), (1, 128), (3, 129), (17, 1000), (64, 4096), (65, 127), (130, 260), (300, 8)])
+def test_quantize_blocks(head, rows, inner, dtype, block_rows, scale_dtype):
+    x = torch.randn((rows, inner), generator=gen(rows * 7 + inner), device="cuda")
+    x *= torch.exp2(torch.randint(-20, 9, (rows, 1), generator=gen(1), device="cuda").float())
+    x = x.to(dtype)
+    q, s = head.quantize_blocks(x, block_rows, scale_dtype)
+    want_q, want_s = quantized(x, block_rows, scale_dtype)
+    assert q.dtype == torch.float8_e4m3fn and q.shape == x.shape and q.stride(0) % 16 == 0
+    assert torch.equal(s.float().double(), want_s)
+    assert torch.equal(q.float().double(), want_q)
+
+
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+def test_quantize_blocks_extremes(head, scale_dtype):
+    x = torch.zeros((8, 256), device="cuda")
+    x[1] = 1e-40  # subnormal: the scale stops at 2^-126
+    x[2, 5], x[2, 6] = float("nan"), 3.0
+    x[3, 5], x[3, 200] = float("inf"), float("-inf")
+    x[4] = 3.4e38
+    x[5, ::2] = -0.0
+    x[6, :128] = torch.tensor([448.0, 1.75, 1.5, 0.0] * 32, device="cuda")  # amax / 448 exactly a power of two
+    x[7, 128:] = float("nan")
+    q, s = head.quantize_blocks(x, 1, scale_dtype)
+    want_q, want_s = quantized(x, 1, scale_dtype)
+    assert torch.equal(s.float().double(), want_s)
+    assert torch.equal(torch.nan_to_num(q.float().double(), nan=1e9), torch.nan_to_num(want_q, nan=1e9))
+    assert s[0, 0].float() == 1 and s[7, 1].float() == 1  # nothing finite but zeros
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_quantize_blocks_strided_and_unaligned(head, dtype):
+    base = torch.randn((40, 700), generator=gen(3), device="cuda").to(dtype)
+    for x in (base[:, 1:301], base[1::3, :256], base.t(), base[:, :300].t(), base[:1, 3:20], base[5].expand(4, 700), base[3]):
+        q, s = head.quantize_blocks(x)
+        want_q, want_s = quantized(x.reshape(-1, x.shape[-1]), 1, F32)
+        assert q.shape == x.shape
+        assert torch.equal(q.float().double().reshape(want_q.shape), want_q) and torch.equal(s.double(), want_s)
+    x = base[:36, :640].reshape(3, 12, 640)
+    q, s = head.quantize_blocks(x)
+    assert q.shape == x.shape and s.shape == (36, 5)
+
+
+def test_quantize_blocks_leaves_its_neighbours(head):
+    """Through the C ABI, into the middle of a wider buffer: of each row only the bytes up to the next multiple of 16."""
+    import tf_faster_rcnn_amd as pkg
+    lib = pkg._lib.lib()
+    x = torch.randn((20, 150), device="cuda")
+    q = torch.full((22, 512), 0xAB, dtype=torch.uint8, device="cuda")
+    s = torch.full((22, 4), -1.0, device="cuda")
+    pkg._lib.check(lib.frcnn_quantize_blocks(x.data_ptr(), 0, 150, 20, 150, 1, q[1].data_ptr() + 16, 512, s[1].data_ptr() + 4, 0, 4, 1,
+                                             torch.cuda.current_stream().cuda_stream))
+    want_q, want_s = quantized(x, 1, F32)
+    assert torch.equal(q[1:21, 16:166].view(torch.float8_e4m3fn).float().double(), want_q)
+    assert (q[1:21, 166:176] == 0).all() and (q[1:21, 176:] == 0xAB).all() and (q[:, :16] == 0xAB).all()
+    assert (q[0] == 0xAB).all() and (q[21] == 0xAB).all()
+    assert torch.equal(s[1:21, 1:3].double(), want_s)
+    assert (s[:, 0] == -1).all() and (s[:, 3] == -1).all() and (s[0] == -1).all() and (s[21] == -1).all()
+
+
+def test_quantize_blocks_empty(head):
+    q, s = head.quantize_blocks(torch.zeros((0, 200), device="cuda"))
+    assert q.shape == (0, 200) and s.shape == (0, 2)
+    q, s = head.quantize_blocks(torch.zeros((5, 0), device="cuda"))
+    assert q.shape == (5, 0) and s.shape == (5, 0)
+
+
+# ---- scaled_matmul --------------------------------------------------------------------------------------------------------------
+def operands(rows, units, inner, scale_dtype, seed=0):
+    g = gen(seed)
+    a = torch.randn((rows, inner), generator=g, device="cuda").clamp_min(-0.3) * torch.exp2(torch.randn((rows, 1), generator=g, device="cuda"))
+    b = torch.randn((units, inner), generator=g, device="cuda") * inner ** -0.5
+    a, sa = quantized(a, 1, scale_dtype)
+    b, sb = quantized(b, 128, scale_dtype)
+    return a.to(torch.float8_e4m3fn), sa.to(scale_dtype), b.to(torch.float8_e4m3fn), sb.to(scale_dtype)
+
+
+def product64(a, sa, b, sb, bias, activation):
+    """The product and the sum of its terms' magnitudes, on the host."""
+    wide = lambda q, s, r: q.float().double().cpu() * s.float().double().cpu().repeat_interleave(r, 0)[:q.shape[0]].repeat_interleave(128, 1)[:, :q.shape[1]]  # noqa: E731
+    x, w = wide(a, sa, 1), wide(b, sb, 128)
+    y, size = x @ w.t().contiguous(), x.abs() @ w.abs().t().contiguous()
+    if bias is not None:
+        y, size = y + bias.double().cpu(), size + bias.double().cpu().abs()
+    return (y.clamp_min(0) if activation == "relu" else y).cuda(), size.cuda()
+
+
+def product_tolerance(y, size, inner, dtype):
+    # fp32 results: products widened to fp16, every sum in fp32.  Others: the e4m3 instructions line the products of a block up
+    # and cut them; they keep more than 12 bits of each (1.1e-5 of the block's sum in the mean, measured)
+    return half_step(dtype) * y.abs() + size * (inner + 8) * U + (0 if dtype == F32 else 2.0 ** -12 * size) + (2.0 ** -24 if dtype == F16 else 0)
+
+
+SHAPES = [(1, 1, 1), (1, 16, 128), (1, 105, 4096), (2, 84, 130), (5, 257, 100), (16, 128, 129), (17, 300, 511), (33, 21, 1024), (64, 64, 2000),
+          (65, 129, 384), (129, 130, 640), (300, 105, 4096), (257, 260, 1000), (300, 4096, 512), (520, 1030, 900), (1000, 512, 256)]
+
+
+@pytest.mark.parametrize("out_dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+@pytest.mark.parametrize("rows,units,inner", SHAPES)
+def test_scaled_matmul(head, rows, units, inner, scale_dtype, out_dtype):
+    a, sa, b, sb = operands(rows, units, inner, scale_dtype, rows + units + inner)
+    bias = torch.randn((units,), generator=gen(5), device="cuda")
+    for bias_, activation in ((None, None), (bias, "relu")):
+        y = head.scaled_matmul(a, sa, b, sb, bias=bias_, activation=activation, out_dtype=out_dtype)
+        want, size = product64(a, sa, b, sb, bias_, activation)
+        assert y.shape == (rows, units) and y.dtype == out_dtype
+        worst = ((y.double() - want).abs() - product_tolerance(want, size, inner, out_dtype)).max().item()
+        assert worst <= 0, (worst, bias_ is not None)
+        assert torch.equal(y, head.scaled_matmul(a, sa, b, sb, bias=bias_, activation=activation, out_dtype=out_dtype))
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,units,inner", [(1, 4096, 28224), (300, 4096, 28224), (4800, 4096, 1152), (4800, 4096, 4100), (2400, 1111, 2050)])
+def test_scaled_matmul_of_the_heads_sizes(head, rows, units, inner, out_dtype):
+    a, sa, b, sb = operands(rows, units, inner, F32, 3)
+    y = head.scaled_matmul(a, sa, b, sb, activation="relu", out_dtype=out_dtype)
+    pick = torch.arange(0, rows, max(1, rows // 37), device="cuda")
+    pick = torch.unique(torch.cat([pick, torch.tensor([rows - 1], device="cuda")]))
+    want, size = product64(a.view(torch.uint8)[pick].view(torch.float8_e4m3fn), sa[pick], b, sb, None, "relu")
+    assert ((y[pick].double() - want).abs() - product_tolerance(want, size, inner, out_dtype)).max().item() <= 0
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [3, 70, 400])
+def test_scaled_matmul_takes_any_layout(head, rows, out_dtype):
+    a, sa, b, sb = operands(rows, 140, 300, F32, 8)
+    want = head.scaled_matmul(a, sa, b, sb, out_dtype=out_dtype)
+    poison = lambda q: torch.full((q.shape[0] + 1, 352), 0x7F, dtype=torch.uint8, device="cuda")  # noqa: E731  (e4m3's NaN)
+    for shift in (0, 16, 5):  # rows in a wider buffer, aligned and not; what lies around them must not be read into the sums
+        wide_a, wide_b = poison(a), poison(b)
+        wide_a[:-1, shift:shift + 300], wide_b[:-1, shift:shift + 300] = a.view(torch.uint8), b.view(torch.uint8)
+        va, vb = (w[:-1, shift:shift + 300].view(torch.float8_e4m3fn) for w in (wide_a, wide_b))
+        assert torch.equal(head.scaled_matmul(va, sa, vb, sb, out_dtype=out_dtype), want)
+    assert torch.equal(head.scaled_matmul(a, sa.contiguous(), b, sb.t().contiguous().t(), out_dtype=out_dtype), want)
+    assert torch.equal(head.scaled_matmul(a.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn), sa, b, sb, out_dtype=out_dtype), want)
+    assert torch.equal(head.scaled_matmul(a, sa[:, :1].expand(-1, 3), b, sb, out_dtype=out_dtype),
+                       head.scaled_matmul(a, sa[:, :1].repeat(1, 3), b, sb, out_dtype=out_dtype))
+    if rows == 70:
+        y = head.scaled_matmul(a.contiguous().view(7, 10, 300), sa, b, sb, out_dtype=out_dtype)
+        assert y.shape == (7, 10, 140) and torch.equal(y.view(70, 140), want)
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [2, 300])
+def test_scaled_matmul_poisoned_rows_stay_alone(head, rows, out_dtype):
+    a, sa, b, sb = operands(rows, 200, 400, F32, 2)
+    clean = head.scaled_matmul(a, sa, b, sb, out_dtype=out_dtype)
+    a.view(torch.uint8)[1, 7] = 0x7F  # NaN
+    b.view(torch.uint8)[150, 399] = 0xFF
+    y = head.scaled_matmul(a, sa, b, sb, activation="relu", out_dtype=out_dtype)
+    bad = torch.isnan(y)
+    assert bad[1].all() and bad[:, 150].all() and bad.sum().item() == 200 + rows - 1
+    assert torch.equal(y[~bad], clean[~bad].clamp_min(0))
+
+
+def test_scaled_matmul_e8m0_special_scales(head):
+    a, sa, b, sb = operands(4, 20, 256, E8M0, 2)
+    s = sa.view(torch.uint8)
+    s[1, 0] = 255  # NaN
+    for out_dtype in (F32, BF16):
+        y = head.scaled_matmul(a, sa, b, sb, out_dtype=out_dtype)
+        assert torch.isnan(y[1]).all() and torch.isfinite(y[[0, 2, 3]]).all()
+
+
+def test_scaled_matmul_empty(head):
+    a, sa, b, sb = operands(3, 20, 128, F32)
+    bias = torch.arange(-3.0, 17.0, device="cuda")
+    none = torch.zeros((3, 0), dtype=torch.float8_e4m3fn, device="cuda")
+    y = head.scaled_matmul(none, torch.zeros((3, 0), device="cuda"), torch.zeros((20, 0), dtype=torch.float8_e4m3fn, device="cuda"),
+                           torch.zeros((1, 0), device="cuda"), bias=bias, activation="relu")
+    assert torch.equal(y, bias.clamp_min(0).bfloat16().expand(3, 20))
+    assert head.scaled_matmul(a[:0], sa[:0], b, sb).shape == (0, 20)
+    assert head.scaled_matmul(a, sa, b[:0], sb[:0]).shape == (3, 0)
+
+
+# ---- group_norm -------------------------------------------------------------------------------------------------------------------
+def norm64(x, gamma, beta, groups, eps, activation, dy=None):
+    """y, stats, dx, dgamma, dbeta in 64 bits, and the magnitudes that their tolerances are made of."""
+    n, c = x.shape[0], x.shape[-1]
+    v = x.double().reshape(n, -1, groups, c // groups)
+    mean = v.mean((1, 3), keepdim=True)
+    var = ((v - mean) ** 2).mean((1, 3), keepdim=True)
+    rstd = 1 / torch.sqrt(var + eps)
+    g, b = gamma.double().view(groups, -1), beta.double().view(groups, -1)
+    xhat = (v - mean) * rstd
+    z = xhat * g + b
+    sig = torch.sigmoid(z)
+    y = {"relu": z.clamp_min(0), "swish": z * sig, None: z}[activation]
+    # fp32: mean is off by (depth of its sum + 2) U of the mean magnitude; xhat by that times rstd and a few U of itself
+    size = v.abs().mean((1, 3), keepdim=True) + mean.abs()
+    off_xhat = 80 * U * (size * rstd + 1 + xhat.abs())
+    off_z = off_xhat * g.abs() + 4 * U * (z.abs() + b.abs())
+    out = {"y": y.reshape(x.shape), "stats": torch.stack([mean.view(n, groups), rstd.view(n, groups)], -1),
+           "off_y": ((1.1 if activation == "swish" else 1) * off_z + (8 * U * z.abs() * (1 + z.abs()) if activation == "swish" else 0)).reshape(x.shape),
+           "off_stats": torch.stack([80 * U * size.view(n, groups), 80 * U * (rstd * (1 + size * rstd)).view(n, groups)], -1)}
+    if dy is not None:
+        d = dy.double().reshape(v.shape)
+        slope = {"relu": (z > 0).double(), "swish": sig * (1 + z * (1 - sig)), None: torch.ones_like(z)}[activation]
+        dz = d * slope
+        # |swish''| <= 0.5; exp2 and rcp cost a few U
+        off_dz = d.abs() * ((0.5 * off_z + 16 * U * (1 + z.abs())) if activation == "swish" else 0)
+        e = dz * g
+        e1, e2 = e.mean((1, 3), keepdim=True), (e * xhat).mean((1, 3), keepdim=True)
+        out["dx"] = (rstd * (e - e1 - xhat * e2)).reshape(x.shape)
+        off_e = off_dz * g.abs() + 4 * U * e.abs()
+        mean_abs = lambda t: t.abs().mean((1, 3), keepdim=True)  # noqa: E731
+        off_e1 = mean_abs(off_e) + 80 * U * mean_abs(e)
+        off_e2 = mean_abs(off_e * xhat.abs()) + mean_abs(e * off_xhat) + 80 * U * mean_abs(e * xhat)
+        out["off_dx"] = (rstd * (off_e + off_e1 + xhat.abs() * off_e2 + off_xhat * e2.abs()) + 80 * U * (1 + size * rstd) * rstd
+                         * (e.abs() + e1.abs() + (xhat * e2).abs())).reshape(x.shape)
+        over = lambda t: t.sum((0, 1)).reshape(-1)  # noqa: E731
+        depth = 80 + v.shape[0] / 64 + 40  # a thread's images in turn, the rows, the workgroups' sums
+        out["dgamma"], out["dbeta"] = over(dz * xhat), over(dz)
+        out["off_dgamma"] = over(off_dz * xhat.abs() + dz.abs() * off_xhat) + depth * U * over((dz * xhat).abs())
+        out["off_dbeta"] = over(off_dz) + depth * U * over(dz.abs())
+    return out
+
+
+def check_norm(got, want, off, dtype, what):
+    worst = ((got.double() - want).abs() - off - half_step(dtype) * want.abs() - (2.0 ** -25 if dtype == F16 else 0)).max().item()
+    assert worst <= 0, (what, worst)
+
+
+NORMS = [((1, 1, 1), 1), ((2, 1, 8), 8), ((3, 5, 7), 7), ((2, 3, 3, 6), 2), ((5, 7, 7, 32), 4), ((3, 7, 7, 64), 32), ((2, 31, 31, 512), 32),
+         ((1, 32, 32, 576), 32), ((2, 32, 32, 576), 1), ((7, 49, 576), 576), ((40, 7, 7, 256), 32), ((1, 20000, 24), 3), ((2, 9001, 23), 1),
+         ((1, 700, 1024), 1), ((3, 2, 2048), 1), ((2, 4, 513), 3), ((3000, 2, 16), 2), ((1, 63, 63, 72), 4)]
+
+
+@pytest.mark.parametrize("activation", [None, "relu", "swish"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape,groups", NORMS)
+def test_group_norm(head, shape, groups, dtype, activation):
+    g = gen(sum(shape) + groups)
+    c = shape[-1]
+    x = (torch.randn(shape, generator=g, device="cuda") + torch.randn((c,), generator=g, device="cuda")).to(dtype)
+    gamma = 1 + 0.3 * torch.randn((c,), generator=g, device="cuda")
+    beta = 0.3 * torch.randn((c,), generator=g, device="cuda")
+    dy = torch.randn(shape, generator=g, device="cuda").to(dtype)
+    if activation == "relu":  # the gate's border: no gradient comes in where rounding may decide it
+        r = norm64(x, gamma, beta, groups, 1e-3, None)
+        dy = torch.where(r["y"].abs() > 4 * r["off_y"], dy.double(), 0.0).to(dtype)
+    r = norm64(x, gamma, beta, groups, 1e-3, activation, dy)
+    y, stats = head.group_norm(x, gamma, beta, groups, activation=activation, return_stats=True)
+    assert y.shape == x.shape and y.dtype == dtype
+    check_norm(y, r["y"], r["off_y"], dtype, "y")
+    check_norm(stats, r["stats"], r["off_stats"], F32, "stats")
+    assert torch.equal(y, head.group_norm(x, gamma, beta, groups, activation=activation))
+    dx, dgamma, dbeta = head.group_norm_gradients(dy, x, gamma, beta, stats, activation=activation)
+    assert dx.shape == x.shape and dx.dtype == dtype
+    check_norm(dx, r["dx"], r["off_dx"], dtype, "dx")
+    check_norm(dgamma, r["dgamma"], r["off_dgamma"], F32, "dgamma")
+    check_norm(dbeta, r["dbeta"], r["off_dbeta"], F32, "dbeta")
+    again = head.group_norm_gradients(dy, x, gamma, beta, stats, activation=activation)
+    assert torch.equal(dx, again[0]) and torch.equal(dgamma, again[1]) and torch.equal(dbeta, again[2])
+
+
+@pytest.mark.parametrize("shape,groups", [((3, 7, 7, 64), 8), ((1, 9000, 64), 4)])
+def test_group_norm_far_from_zero(head, shape, groups):
+    """Means a thousand deviations away: the variance is that of the centred values."""
+    x = torch.randn(shape, generator=gen(1), device="cuda") + 1000.0
+    c = shape[-1]
+    gamma, beta = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+    r = norm64(x, gamma, beta, groups, 1e-3, None)
+    y, stats = head.group_norm(x, gamma, beta, groups, return_stats=True)
+    check_norm(y, r["y"], r["off_y"], F32, "y")
+    # one-pass sums of squares would lose 1000^2 * 2^-24 = 6 % of the variance
+    assert ((stats[..., 1].double() - r["stats"][..., 1]).abs() < 1e-4).all()
+    x = torch.full(shape, 7.0, device="cuda")  # no variance at all
+    y = head.group_norm(x, gamma, beta + 0.25, groups)
+    assert ((y - 0.25).abs() <= 80 * U * 14 * 1e-3 ** -0.5).all()
+
+
+@pytest.mark.parametrize("shape,groups", [((3, 7, 7, 64), 8), ((2, 9000, 64), 8)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_group_norm_poison_stays_in_its_group(head, shape, groups, value):
+    x = torch.randn(shape, generator=gen(1), device="cuda")
+    gamma, beta = torch.ones(shape[-1], device="cuda"), torch.zeros(shape[-1], device="cuda")
+    clean = head.group_norm(x, gamma, beta, groups, activation="relu")
+    flat = x.view(shape[0], -1, groups, shape[-1] // groups)
+    flat[1, 30, 2, 3] = value
+    y = head.group_norm(x, gamma, beta, groups, activation="relu").view(flat.shape)
+    assert torch.isnan(y[1, :, 2]).any()
+    keep = torch.ones_like(y, dtype=torch.bool)
+    keep[1, :, 2] = False
+    assert torch.equal(y[keep], clean.view(flat.shape)[keep])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_group_norm_strided_and_unaligned(head, dtype):
+    base = torch.randn((6, 9, 9, 70), generator=gen(4), device="cuda").to(dtype)
+    gamma, beta = torch.randn(64, device="cuda"), torch.randn(64, device="cuda")
+    for x in (base[..., 3:67], base[:, ::2, ::2, :64], base.permute(0, 2, 1, 3)[..., :64], base.view(-1)[1:1 + 6 * 64].view(6, 1, 64)):
+        want = head.group_norm(x.contiguous().clone(), gamma, beta, 8)
+        got = head.group_norm(x, gamma, beta, 8)
+        # an unaligned tensor takes element loads, whose sums run in another order
+        r = norm64(x.contiguous(), gamma, beta, 8, 1e-3, None)
+        check_norm(got, r["y"], r["off_y"], dtype, "y")
+        check_norm(want, r["y"], r["off_y"], dtype, "y")
+
+
+def test_group_norm_gradients_against_differences(head):
+    x = torch.randn((2, 6, 12), generator=gen(1), device="cuda", dtype=torch.float64)
+    gamma, beta = 1 + 0.1 * torch.randn(12, generator=gen(2), device="cuda"), torch.randn(12, generator=gen(3), device="cuda")
+    w = torch.randn(x.shape, generator=gen(4), device="cuda", dtype=torch.float64)
+    for activation in (None, "swish"):
+        leaves = [t.clone().requires_grad_() for t in (x.float(), gamma, beta)]
+        y = head.group_norm(leaves[0], leaves[1], leaves[2], 3, activation=activation)
+        y.backward(w.float())
+        loss = lambda a, b, c: (norm64(a, b, c, 3, 1e-3, activation)["y"] * w).sum()  # noqa: E731
+        h = 1e-5
+        for leaf, at in zip(leaves, range(3)):
+            args = [x.float().double(), gamma.double(), beta.double()]
+            for i in range(0, leaf.numel(), 5):
+                up, down = [t.clone() for t in args], [t.clone() for t in args]
+                up[at].view(-1)[i] += h
+                down[at].view(-1)[i] -= h
+                slope = (loss(*up) - loss(*down)) / (2 * h)
+                # central differences in 64 bits: h^2 of the third derivative and 1e-16 / h; the gradient itself is fp32
+                assert abs(leaf.grad.view(-1)[i].item() - slope.item()) < 1e-5 * (1 + abs(slope.item()) + w.abs().sum().item() / 10)
+
+
+def test_group_norm_empty_batch(head):
+    x = torch.zeros((0, 7, 7, 64), device="cuda", requires_grad=True)
+    gamma, beta = (torch.ones(64, device="cuda", requires_grad=True) for _ in range(2))
+    y = head.group_norm(x, gamma, beta, 8)
+    assert y.shape == x.shape
+    y.sum().backward()
+    assert (gamma.grad == 0).all() and (beta.grad == 0).all() and x.grad.shape == x.shape
+
+
+# ---- dropout ------------------------------------------------------------------------------------------------------------------------
+def philox(blocks, seed, offset):
+    """Philox4x32 with 7 rounds, in Python's integers through NumPy's uint64."""
+    mask, half = np.uint64(0xFFFFFFFF), np.uint64(32)
+    index = np.asarray(blocks, dtype=np.uint64)
+    c = [index & mask, index >> half, np.full_like(index, offset & 0xFFFFFFFF), np.full_like(index, offset >> 32)]
+    for r in range(7):
+        k0, k1 = np.uint64((seed + r * 0x9E3779B9) & 0xFFFFFFFF), np.uint64(((seed >> 32) + r * 0xBB67AE85) & 0xFFFFFFFF)
+        p, q = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(q >> half) ^ c[1] ^ k0, q & mask, (p >> half) ^ c[3] ^ k1, p & mask]
+    return np.stack(c, axis=-1)
+
+
+def dropped(x, rate, seed, offset):
+    words = philox(np.arange(-(-x.numel() // 4)), seed, offset).reshape(-1)[:x.numel()]
+    keep = torch.from_numpy(words >= np.uint64(round(rate * 2 ** 32))).cuda().view(x.shape)
+    return torch.where(keep, x.float() * float(np.float32(1 / (1 - rate))), 0.0).to(x.dtype)
+
+
+def test_philox_known_answers():
+    # counter and key all zeros, all ones: the published vectors for 7 rounds
+    assert [hex(v) for v in philox([0], 0, 0)[0]] == ["0x5f6fb709", "0xd893f64", "0x4f121f81", "0x4f730a48"]
+    assert [hex(v) for v in philox([2 ** 64 - 1], 2 ** 64 - 1, 2 ** 64 - 1)[0]] == ["0x5207ddc2", "0x45165e59", "0x4d8ee751", "0x8c52f662"]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("count", [1, 3, 4, 7, 8, 9, 255, 1000, 65536, 300 * 4096 + 5])
+def test_dropout(head, count, dtype):
+    x = torch.randn((count,), generator=gen(count), device="cuda").to(dtype)
+    for rate, seed, offset in ((0.5, 1, 0), (0.1, 2 ** 64 - 3, 2 ** 63 + 5), (0.93, 12345678901234567, 7), (0.0, 3, 3)):
+        y = head.dropout(x, rate, seed, offset)
+        assert y.dtype == dtype and torch.equal(y, dropped(x, rate, seed, offset))
+        state = torch.tensor([(seed + 2 ** 63) % 2 ** 64 - 2 ** 63, (offset + 2 ** 63) % 2 ** 64 - 2 ** 63], device="cuda")
+        assert torch.equal(y, head.dropout(x, rate, state))
+
+
+def test_dropout_rate_and_independence(head):
+    n = 1 << 22
+    x = torch.ones(n, device="cuda")
+    masks = [head.dropout(x, 0.3, 5, i) != 0 for i in range(3)] + [head.dropout(x, 0.3, 6, 0) != 0]
+    for m in masks:  # six deviations of a binomial of n draws
+        assert abs(m.double().mean().item() - 0.7) < 6 * (0.21 / n) ** 0.5
+    for i in range(4):
+        for j in range(i):
+            assert abs((masks[i] & masks[j]).double().mean().item() - 0.49) < 6 * (0.49 * 0.51 / n) ** 0.5
+
+
+def test_dropout_drops_what_is_not_finite(head):
+    x = torch.full((4096,), float("nan"), device="cuda")
+    y = head.dropout(x, 0.5, 9)
+    keep = dropped(torch.ones(4096, device="cuda"), 0.5, 9, 0) != 0
+    assert torch.isnan(y[keep]).all() and (y[~keep] == 0).all()
+    tiny = head.dropout(torch.ones(1 << 20, device="cuda"), 1 - 2.0 ** -40, 1)
+    assert torch.isfinite(tiny).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_dropout_strided_and_unaligned(head, dtype):
+    base = torch.randn((50, 77), generator=gen(2), device="cuda").to(dtype)
+    for x in (base.t(), base[:, 3:40], base[::2], base.view(-1)[1:1000], base.view(-1)[3:3]):
+        assert torch.equal(head.dropout(x, 0.4, 8, 2), dropped(x.contiguous(), 0.4, 8, 2))
+
+
+def test_dropout_gradient(head):
+    x = torch.randn((333, 7), generator=gen(1), device="cuda", requires_grad=True)
+    dy = torch.randn((7, 333), generator=gen(2), device="cuda").t()
+    state = torch.tensor([4, 9], device="cuda")
+    for seed, kw in ((4, {"offset": 9}), (state, {})):
+        x.grad = None
+        y = head.dropout(x, 0.25, seed, **kw)
+        state[1] += 1  # the backward pass must go by what the forward pass used
+        y.backward(dy)
+        state[1] -= 1
+        assert torch.equal(x.grad, dropped(dy.contiguous(), 0.25, 4, 9))
+    # linear: a difference quotient is the gradient itself
+    one = torch.zeros_like(x)
+    one[100, 3] = 1.0
+    assert torch.equal(head.dropout(one, 0.25, 4, 9)[100, 3], dropped(torch.ones((333, 7), device="cuda"), 0.25, 4, 9)[100, 3])
+
+
+# ---- streams, graphs ------------------------------------------------------------------------------------------------------------------
+def chain(head, x, state, weights, out_dtype=BF16):
+    gamma, beta, w, ws, bias = weights
+    y, stats = head.group_norm(x, gamma, beta, 8, activation="swish", return_stats=True)
+    z = head.dropout(y, 0.5, state)
+    q, s = head.quantize_blocks(z.flatten(1))
+    out = head.scaled_matmul(q, s, w, ws, bias=bias, activation="relu", out_dtype=out_dtype)
+    grads = head.group_norm_gradients(head.dropout(x, 0.5, state), x, gamma, beta, stats, activation="swish")
+    return [out, z, *grads]
+
+
+def weights_for(head, inner, units, channels):
+    w, ws = head.quantize_blocks(torch.randn((units, inner), generator=gen(1), device="cuda") * inner ** -0.5, block_rows=128)
+    return (1 + 0.1 * torch.randn(channels, generator=gen(2), device="cuda"), 0.1 * torch.randn(channels, generator=gen(3), device="cuda"), w, ws,
+            torch.randn(units, generator=gen(4), device="cuda"))
+
+
+@pytest.mark.parametrize("shape", [(20, 7, 7, 64), (2, 80, 80, 64)])
+def test_replayed_graphs_equal_eager_calls(head, shape):
+    inner = shape[1] * shape[2] * shape[3]
+    weights = weights_for(head, inner, 264, 64)
+    state = torch.tensor([11, 0], device="cuda")
+    inputs = [torch.randn(shape, generator=gen(i), device="cuda").bfloat16() for i in range(4)]
+    want = []
+    for i, x in enumerate(inputs):
+        state[1] = i
+        want.append([t.clone() for t in chain(head, x, state, weights)])
+    holders = [torch.zeros(shape, dtype=BF16, device="cuda") for _ in range(2)]
+    graphs, outs = [], []
+    for h in holders:  # two graphs captured one after the other: each has scratch memory of its own
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = chain(head, h, state, weights)
+        graphs.append(graph)
+        outs.append(out)
+    for i in range(4):
+        state[1] = i
+        for j in (0, 1):
+            holders[j].copy_(inputs[i])
+        streams = [torch.cuda.Stream() for _ in graphs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):  # replayed at the same time
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        chain(head, inputs[(i + 1) % 4], state, weights)  # the program's own work in between
+        torch.cuda.synchronize()
+        for j in (0, 1):
+            for got, exp in zip(outs[j], want[i]):
+                assert torch.equal(got, exp)
+
+
+def test_captured_backward_beside_an_eager_graph(head):
+    """torch.autograd.grad inside a capture: refused while an eager graph of the same leaves is alive (the capture would be
+    made to wait for that graph's stream, which ends the process), and right once it is gone."""
+    gamma, beta = (torch.ones(64, device="cuda", requires_grad=True) for _ in range(2))
+    x = torch.randn((30, 7, 7, 64), generator=gen(1), device="cuda", requires_grad=True)
+    state = torch.tensor([3, 5], device="cuda")
+
+    def step():
+        y = head.dropout(head.group_norm(x, gamma, beta, 8, activation="swish"), 0.3, state)
+        return torch.autograd.grad(y.float().square().sum(), (x, gamma, beta))
+
+    want = [t.clone() for t in step()]
+    alive = [head.group_norm(x, gamma, beta, 8), head.dropout(x, 0.5, 1)]
+    torch.cuda.synchronize()
+    for call in (lambda: head.group_norm(x, gamma, beta, 8), lambda: head.dropout(x, 0.5, 1)):
+        with pytest.raises(RuntimeError, match="alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    sum(t.sum() for t in alive).backward()
+    del alive
+    x.grad = gamma.grad = beta.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        step()
+
+
+def test_calls_on_two_streams(head):
+    weights = weights_for(head, 49 * 64, 300, 64)
+    state = torch.tensor([11, 0], device="cuda")
+    xs = [torch.randn((200, 7, 7, 64), generator=gen(i), device="cuda").bfloat16() for i in range(2)]
+    want = [chain(head, x, state, weights) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [None, None]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = chain(head, xs[i], state, weights)
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            for a, b in zip(g, w):
+                assert torch.equal(a, b)
+
+
+# ---- the layers, as they are used ------------------------------------------------------------------------------------------------------
+def test_serving_head_between_pooling_and_decoder():
+    """RoIBBox -> RoIPooling -> dense layers in 8-bit floating point -> Decoder, against the head in 64 bits on the same pooled
+    features: an e4m3 operand is off by at most 2^-4 of its value (half a step of 3 fraction bits), or half its smallest step."""
+    import synth
+    import tf_faster_rcnn_amd as pkg
+    B, G, C, L, R = 2, 16, 64, 5, 32
+    hp = pkg.train_utils.get_hyper_params("mobilenet_v2", feature_map_shape=G, pre_nms_topn=1024, test_nms_topn=R)
+    deltas, scores = synth.rpn_outputs(0, B, G)
+    rois = pkg.faster_rcnn.RoIBBox(pkg.bbox_utils.generate_anchors(hp), "inference", hp)([torch.as_tensor(deltas).cuda(), torch.as_tensor(scores).cuda()])
+    maps = pkg.box_head.GroupNormalization(8, activation="relu")(torch.as_tensor(synth.feature_map(0, B, G, C)).cuda()).detach()
+    pooled = pkg.faster_rcnn.RoIPooling(hp)([maps, rois])
+    flat = pooled.flatten(2)
+    g = gen(0)
+    k1, b1 = torch.randn((flat.shape[-1], 256), generator=g, device="cuda") * flat.shape[-1] ** -0.5, 0.1 * torch.randn(256, generator=g, device="cuda")
+    k2, b2 = torch.randn((256, 5 * L), generator=g, device="cuda") * 0.2, torch.zeros(5 * L, device="cuda")
+    fc1 = pkg.box_head.QuantizedDense(256, activation="relu", name="frcnn_fc1")
+    out = pkg.box_head.QuantizedDense(5 * L, scale_dtype=E8M0, out_dtype=F32)
+    fc1.set_weights([k1, b1])
+    out.set_weights([k2, b2])
+    hidden = pkg.box_head.Dropout(0.5)(fc1(flat))
+    logits = out(hidden)
+    assert hidden.shape == (B, R, 256) and logits.shape == (B, R, 5 * L) and logits.dtype == F32
+    want1 = (flat.double() @ k1.double() + b1.double()).clamp_min(0)
+    # both operands of each product are off by 2^-4 at most: (1 + 2^-4)^2 - 1 of the sum of magnitudes, subnormal steps aside
+    size1 = flat.double().abs() @ k1.double().abs()
+    assert ((hidden.double() - want1).abs() <= 0.14 * size1 + 2.0 ** -8 * want1 + 1e-3).all()
+    want2 = hidden.double() @ k2.double()
+    assert ((logits.double() - want2).abs() <= 0.14 * (hidden.double().abs() @ k2.double().abs()) + 1e-3).all()
+    probs = torch.softmax(logits[..., :L], -1)
+    boxes, labels, confidence = pkg.faster_rcnn.Decoder(hp["variances"], L)([rois, logits[..., L:].contiguous(), probs])
+    assert boxes.shape == (B, 200, 4) and torch.isfinite(boxes).all() and (confidence >= 0).all()
+    with pytest.raises(ValueError, match="no gradient"):
+        fc1(flat.requires_grad_())
+
+
+def test_training_head_steps():
+    """GroupNormalization and Dropout on pooled features, eager and captured: gradients by the formula, a new mask at each step."""
+    import tf_faster_rcnn_amd as pkg
+    norm, drop = pkg.box_head.GroupNormalization(8, activation="swish"), pkg.box_head.Dropout(0.4, seed=77)
+    x = torch.randn((12, 7, 7, 64), generator=gen(0), device="cuda", requires_grad=True)
+    with pytest.raises(ValueError):
+        norm.set_weights([torch.ones(4), torch.ones(5)])
+
+    def step():
+        y = drop(norm(x), training=True)
+        return [y.detach(), *torch.autograd.grad(y.sum(), (x, norm.gamma, norm.beta))]
+
+    for i in range(2):
+        got = step()
+        dy = dropped(torch.ones(x.shape, device="cuda"), 0.4, 77, i)
+        r = norm64(x.detach(), norm.gamma.detach(), norm.beta.detach(), 8, 1e-3, "swish", dy)
+        for k, name in enumerate(("dx", "dgamma", "dbeta")):
+            check_norm(got[k + 1], r[name], r["off_" + name], F32, name)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(2, 5):
+        graph.replay()
+        torch.cuda.synchronize()
+        mask = dropped(torch.ones(x.shape, device="cuda"), 0.4, 77, i) != 0
+        assert torch.equal(out[0] != 0, mask & (norm(x).detach() != 0))
+    assert drop(x) is x
+    fresh = pkg.box_head.Dropout(0.4)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fresh(x, training=True)
+    torch.cuda.synchronize()

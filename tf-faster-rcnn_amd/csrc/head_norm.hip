@@ -1,0 +1,794 @@
+// head_norm.hip -- group normalisation of channels-last tensors with an activation, and its gradients.
+//
+// x (N, S, C), C = G groups of Cg channels; per image n and group g, over the m = S * Cg values:
+//   mean, var = E (x - mean)^2, rstd = 1 / sqrt(var + eps), xhat = (x - mean) rstd, z = gamma xhat + beta, y = act(z)
+//   dz = dy act'(z), dgamma = sum dz xhat, dbeta = sum dz, d = gamma dz,
+//   dx = rstd (d - E d - xhat E (d xhat))          (the expectations over the same m values)
+//
+// Bound by memory: x read and y written once; x, dy read and dx written once.  A workgroup takes a slab of channels (whole
+// groups) of one image and keeps it in registers, so the variance is that of the centred values (no cancellation) and the
+// data is read once.  Where a slab of one image does not fit a workgroup's registers the positions are cut into chunks:
+// statistics per chunk, joined in a fixed order (Chan, Golub and LeVeque's update), then a second pass over the data.
+//
+// A thread owns one pack of channels (a column) and walks the positions.  Sums are kept per channel -- a pack may straddle
+// groups -- added over the workgroup's rows in LDS by halving, then over the channels of each group by lanes of one wave.
+// No atomics: results do not depend on the order in which workgroups run.
+#include "head_common.hpp"
+
+namespace frcnn {
+
+enum { kActNone = FRCNN_ACT_NONE, kActRelu = FRCNN_ACT_RELU, kActSwish = FRCNN_ACT_SWISH };
+
+__device__ __forceinline__ float sigmoid_fast(float z) {  // exp2 and rcp are good to one unit in the last place each
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == kActRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
+  if (act == kActSwish) return z * sigmoid_fast(z);
+  return z;
+}
+
+__device__ __forceinline__ float activate_grad(float dy, float z, int act) {
+  if (act == kActRelu) return z > 0.0f ? dy : 0.0f;
+  if (act == kActSwish) {
+    const float s = sigmoid_fast(z);
+    return dy * (s * __builtin_fmaf(z, 1.0f - s, 1.0f));
+  }
+  return dy;
+}
+
+struct NormShape {
+  int N, S, C, G, Cg;
+  int slab;    // channels per workgroup, whole groups; the last slab of a row may be shorter
+  int slabs;   // ceil(C / slab)
+  int chunk;   // positions per workgroup
+  int chunks;  // ceil(S / chunk)
+};
+
+// ---- reductions inside a workgroup ---------------------------------------------------------------------------------------
+// red[rows][slab]: sum over the rows, into row 0.  `row` < rows are the threads that own data; halving keeps the order fixed.
+template <int VEC, int K>
+__device__ __forceinline__ void rows_to_first(float *red, int rows, int slab, int row, int col, bool active, float (&v)[K][VEC]) {
+  // each of the K sums has its own plane of rows * slab floats
+  const int plane = rows * slab;
+  if (active)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) red[k * plane + row * slab + col + e] = v[k][e];
+  int n = rows;
+  while (n > 1) {
+    const int half = (n + 1) >> 1;
+    __syncthreads();
+    if (active && row + half < n)
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          v[k][e] += red[k * plane + (row + half) * slab + col + e];
+          red[k * plane + row * slab + col + e] = v[k][e];
+        }
+    n = half;
+  }
+  __syncthreads();
+}
+
+// out[g] = sum of weight(c) * chan[c] over the group's channels; P lanes (a power of two <= 64) per group.
+template <typename F>
+__device__ __forceinline__ void groups_of(int groups, int Cg, int threads, F value, float *out) {
+  int P = 1;
+  while (P < Cg && P < 64) P <<= 1;
+  const int per = threads / P;
+  const int sub = threadIdx.x & (P - 1), first = threadIdx.x / P;
+  for (int base = 0; base < groups; base += per) {
+    const int g = base + first;
+    float s = 0.0f;
+    if (g < groups)
+      for (int c = sub; c < Cg; c += P) s += value(g * Cg + c);
+    for (int d = P >> 1; d > 0; d >>= 1) s += __shfl_xor(s, d);
+    if (g < groups && sub == 0) out[g] = s;
+  }
+  __syncthreads();
+}
+
+template <typename T, int VEC, int NT>
+struct Column {  // a thread's place in the slab
+  int row, col, rows;  // first row, first channel of its pack inside the slab, rows per pass
+  int width;           // channels of this slab
+  bool active;
+  __device__ __forceinline__ Column(const NormShape &s, int slab_index) {
+    width = min(s.slab, s.C - slab_index * s.slab);
+    const int vc = s.slab / VEC;  // the same for every slab, also a shorter last one
+    rows = NT / vc;
+    row = (int)threadIdx.x / vc;
+    col = ((int)threadIdx.x - row * vc) * VEC;
+    active = row < rows && col < width;
+  }
+};
+
+// ---- forward, a slab of one image (or one chunk of it) in registers --------------------------------------------------------
+// WRITE: apply and write y (the whole image is here: chunks == 1).  Otherwise only the chunk's mean and the sum of its
+// squared deviations go to `part` (N, chunks, G, 2).
+template <typename T, int VEC, int NV, int NT, bool WRITE>
+__global__ __launch_bounds__(NT) void norm_resident_kernel(const T *__restrict__ x, T *__restrict__ y, const float *__restrict__ gamma,
+                                                           const float *__restrict__ beta, float *__restrict__ stats, NormShape s,
+                                                           float eps, int act) {
+  extern __shared__ float lds[];
+  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
+  const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
+  const int chunk_index = rest % s.chunks, n = rest / s.chunks;
+  const Column<T, VEC, NT> me(s, slab_index);
+  const int c0 = slab_index * s.slab + me.col;
+  const int p0 = chunk_index * s.chunk;
+  const int count = min(s.chunk, s.S - p0);
+  const long long base = ((long long)n * s.S + p0) * s.C + c0;
+  const int groups = me.width / s.Cg;
+  float *red = lds, *gsum = lds + me.rows * s.slab, *grstd = gsum + s.slab / s.Cg;
+
+  Pack<T, VEC> v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = me.row + i * me.rows;
+    v[i] = (me.active && p < count) ? Pack<T, VEC>::load(x + base + (long long)p * s.C) : Pack<T, VEC>::zero();
+  }
+  int group[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) group[e] = me.active ? (me.col + e) / s.Cg : 0;
+
+  float sum[1][VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sum[0][e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float f[VEC];
+    v[i].unpack(f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum[0][e] += f[e];  // rows beyond the end hold zeros
+  }
+  rows_to_first<VEC, 1>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
+  const float inv = 1.0f / ((float)count * (float)s.Cg);
+  groups_of(groups, s.Cg, NT, [&](int c) { return red[c]; }, gsum);
+
+  float mean[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) mean[e] = gsum[group[e]] * inv;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sum[0][e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (me.row + i * me.rows < count) {
+      float f[VEC];
+      v[i].unpack(f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = f[e] - mean[e];
+        sum[0][e] = __builtin_fmaf(d, d, sum[0][e]);
+      }
+    }
+  }
+  rows_to_first<VEC, 1>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
+  groups_of(groups, s.Cg, NT, [&](int c) { return red[c]; }, grstd);
+
+  const int g0 = slab_index * s.slab / s.Cg;
+  if constexpr (!WRITE) {
+    float *part = stats + (((long long)n * s.chunks + chunk_index) * s.G + g0) * 2;
+    for (int g = threadIdx.x; g < groups; g += NT) {
+      part[2 * g] = gsum[g] * inv;
+      part[2 * g + 1] = grstd[g];
+    }
+  } else {
+    if (stats) {
+      float *out = stats + ((long long)n * s.G + g0) * 2;
+      for (int g = threadIdx.x; g < groups; g += NT) {
+        out[2 * g] = gsum[g] * inv;
+        out[2 * g + 1] = 1.0f / __builtin_sqrtf(__builtin_fmaf(grstd[g], inv, eps));
+      }
+    }
+    if (!me.active) return;
+    float a[VEC], b[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      a[e] = gamma[c0 + e] / __builtin_sqrtf(__builtin_fmaf(grstd[group[e]], inv, eps));
+      b[e] = beta[c0 + e];
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = me.row + i * me.rows;
+      if (p < count) {
+        float f[VEC];
+        v[i].unpack(f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = activate(__builtin_fmaf(f[e] - mean[e], a[e], b[e]), act);
+        Pack<T, VEC>::store(y + base + (long long)p * s.C, f);
+      }
+    }
+  }
+}
+
+// Joins the chunks' statistics: one wave per (image, group); the chunks a lane takes and the order of the joins are fixed.
+__device__ __forceinline__ void join_stats(float &mean, float &m2, float &have, float mean_b, float m2_b, float count_b) {
+  if (count_b == 0.0f) return;
+  if (have == 0.0f) {
+    mean = mean_b, m2 = m2_b, have = count_b;
+    return;
+  }
+  const float d = mean_b - mean, total = have + count_b, w = count_b / total;
+  mean = __builtin_fmaf(d, w, mean);
+  m2 += __builtin_fmaf(d * d, have * w, m2_b);
+  have = total;
+}
+
+__global__ __launch_bounds__(256) void norm_join_kernel(const float *__restrict__ part, float *__restrict__ stats, NormShape s, float eps) {
+  const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= (long long)s.N * s.G) return;
+  const long long n = i / s.G;
+  const int g = (int)(i - n * s.G);
+  float mean = 0.0f, m2 = 0.0f, have = 0.0f;
+  for (int c = lane_id(); c < s.chunks; c += 64) {
+    const f32x2 p = *reinterpret_cast<const f32x2 *>(part + ((n * s.chunks + c) * s.G + g) * 2);
+    join_stats(mean, m2, have, p.x, p.y, (float)min(s.chunk, s.S - c * s.chunk) * (float)s.Cg);
+  }
+  for (int d = 32; d > 0; d >>= 1) {
+    const float mean_b = __shfl_xor(mean, d), m2_b = __shfl_xor(m2, d), have_b = __shfl_xor(have, d);
+    join_stats(mean, m2, have, mean_b, m2_b, have_b);
+  }
+  if (lane_id() == 0) {
+    stats[2 * i] = mean;
+    stats[2 * i + 1] = 1.0f / __builtin_sqrtf(m2 / have + eps);
+  }
+}
+
+// y from x and the joined statistics; the thread layout of norm_resident_kernel.
+template <typename T, int VEC, int NT>
+__global__ __launch_bounds__(NT) void norm_apply_kernel(const T *__restrict__ x, T *__restrict__ y, const float *__restrict__ gamma,
+                                                        const float *__restrict__ beta, const float *__restrict__ stats, NormShape s,
+                                                        int act) {
+  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
+  const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
+  const int chunk_index = rest % s.chunks, n = rest / s.chunks;
+  const Column<T, VEC, NT> me(s, slab_index);
+  if (!me.active) return;
+  const int c0 = slab_index * s.slab + me.col;
+  const int p0 = chunk_index * s.chunk;
+  const int count = min(s.chunk, s.S - p0);
+  const long long base = ((long long)n * s.S + p0) * s.C + c0;
+  float mean[VEC], a[VEC], b[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const float *st = stats + ((long long)n * s.G + (c0 + e) / s.Cg) * 2;
+    mean[e] = st[0];
+    a[e] = gamma[c0 + e] * st[1];
+    b[e] = beta[c0 + e];
+  }
+#pragma unroll 4
+  for (int p = me.row; p < count; p += me.rows) {
+    float f[VEC];
+    Pack<T, VEC>::load(x + base + (long long)p * s.C).unpack(f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = activate(__builtin_fmaf(f[e] - mean[e], a[e], b[e]), act);
+    Pack<T, VEC>::store(y + base + (long long)p * s.C, f);
+  }
+}
+
+// ---- gradients -------------------------------------------------------------------------------------------------------------
+template <int VEC>
+struct GradCoefficients {
+  float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC];
+  __device__ __forceinline__ void load(const float *__restrict__ stats, const float *__restrict__ g, const float *__restrict__ b,
+                                       const NormShape &s, int n, int c0) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float *st = stats + ((long long)n * s.G + (c0 + e) / s.Cg) * 2;
+      mean[e] = st[0];
+      rstd[e] = st[1];
+      gamma[e] = g[c0 + e];
+      beta[e] = b[c0 + e];
+    }
+  }
+  // xhat and dz of one element
+  __device__ __forceinline__ void of(int e, float x, float dy, int act, float &xhat, float &dz) const {
+    xhat = (x - mean[e]) * rstd[e];
+    dz = activate_grad(dy, __builtin_fmaf(xhat, gamma[e], beta[e]), act);
+  }
+};
+
+// A slab of one image's x and dy in registers; each workgroup takes `per` images in turn and leaves its sums for dgamma and
+// dbeta in sums (workgroups along N, C, 2).
+template <typename T, int VEC, int NV, int NT>
+__global__ __launch_bounds__(NT) void norm_grad_resident_kernel(const T *__restrict__ dy, const T *__restrict__ x,
+                                                                const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                                const float *__restrict__ stats, T *__restrict__ dx,
+                                                                float *__restrict__ sums, NormShape s, int per, int act) {
+  extern __shared__ float lds[];
+  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
+  const int part = (int)(blockIdx.x / (unsigned)s.slabs);
+  const Column<T, VEC, NT> me(s, slab_index);
+  const int c0 = slab_index * s.slab + me.col;
+  const int groups = me.width / s.Cg;
+  float *red = lds, *first = lds + 2 * me.rows * s.slab, *second = first + s.slab / s.Cg, *weight = second + s.slab / s.Cg;
+  const int plane = me.rows * s.slab;
+  for (int c = threadIdx.x; c < me.width; c += NT) weight[c] = gamma[slab_index * s.slab + c];
+  int group[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) group[e] = me.active ? (me.col + e) / s.Cg : 0;
+  float total[2][VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) total[0][e] = total[1][e] = 0.0f;
+  const float inv = 1.0f / ((float)s.S * (float)s.Cg);
+
+  const int last = min(s.N, (part + 1) * per);
+  for (int n = part * per; n < last; ++n) {
+    const long long base = (long long)n * s.S * s.C + c0;
+    Pack<T, VEC> vx[NV], vd[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = me.row + i * me.rows;
+      const bool in = me.active && p < s.S;
+      vx[i] = in ? Pack<T, VEC>::load(x + base + (long long)p * s.C) : Pack<T, VEC>::zero();
+      vd[i] = in ? Pack<T, VEC>::load(dy + base + (long long)p * s.C) : Pack<T, VEC>::zero();
+    }
+    GradCoefficients<VEC> k;
+    if (me.active) k.load(stats, gamma, beta, s, n, c0);
+    float sum[2][VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum[0][e] = sum[1][e] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (me.row + i * me.rows < s.S) {
+        float fx[VEC], fd[VEC];
+        vx[i].unpack(fx);
+        vd[i].unpack(fd);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          float xhat, dz;
+          k.of(e, fx[e], fd[e], act, xhat, dz);
+          sum[0][e] += dz;
+          sum[1][e] = __builtin_fmaf(dz, xhat, sum[1][e]);
+        }
+      }
+    }
+    rows_to_first<VEC, 2>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
+    if (me.active && me.row == 0)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        total[0][e] += sum[0][e];
+        total[1][e] += sum[1][e];
+      }
+    groups_of(groups, s.Cg, NT, [&](int c) { return red[c] * weight[c]; }, first);
+    groups_of(groups, s.Cg, NT, [&](int c) { return red[plane + c] * weight[c]; }, second);
+    if (me.active) {
+      float d1[VEC], d2[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        d1[e] = first[group[e]] * inv;
+        d2[e] = second[group[e]] * inv;
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int p = me.row + i * me.rows;
+        if (p < s.S) {
+          float fx[VEC], fd[VEC];
+          vx[i].unpack(fx);
+          vd[i].unpack(fd);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            float xhat, dz;
+            k.of(e, fx[e], fd[e], act, xhat, dz);
+            fd[e] = k.rstd[e] * (__builtin_fmaf(dz, k.gamma[e], -d1[e]) - xhat * d2[e]);
+          }
+          Pack<T, VEC>::store(dx + base + (long long)p * s.C, fd);
+        }
+      }
+    }
+    __syncthreads();  // red, first and second are free for the next image
+  }
+  if (me.active && me.row == 0)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float *o = sums + ((long long)part * s.C + c0 + e) * 2;
+      o[0] = total[0][e];
+      o[1] = total[1][e];
+    }
+}
+
+// Per-channel sums of one chunk of positions, into sums (N, chunks, C, 2).
+template <typename T, int VEC, int NT>
+__global__ __launch_bounds__(NT) void norm_grad_sums_kernel(const T *__restrict__ dy, const T *__restrict__ x,
+                                                            const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                            const float *__restrict__ stats, float *__restrict__ sums, NormShape s,
+                                                            int act) {
+  extern __shared__ float lds[];
+  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
+  const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
+  const int chunk_index = rest % s.chunks, n = rest / s.chunks;
+  const Column<T, VEC, NT> me(s, slab_index);
+  const int c0 = slab_index * s.slab + me.col;
+  const int p0 = chunk_index * s.chunk;
+  const int count = min(s.chunk, s.S - p0);
+  const long long base = ((long long)n * s.S + p0) * s.C + c0;
+  float sum[2][VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sum[0][e] = sum[1][e] = 0.0f;
+  if (me.active) {
+    GradCoefficients<VEC> k;
+    k.load(stats, gamma, beta, s, n, c0);
+#pragma unroll 4
+    for (int p = me.row; p < count; p += me.rows) {
+      float fx[VEC], fd[VEC];
+      Pack<T, VEC>::load(x + base + (long long)p * s.C).unpack(fx);
+      Pack<T, VEC>::load(dy + base + (long long)p * s.C).unpack(fd);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float xhat, dz;
+        k.of(e, fx[e], fd[e], act, xhat, dz);
+        sum[0][e] += dz;
+        sum[1][e] = __builtin_fmaf(dz, xhat, sum[1][e]);
+      }
+    }
+  }
+  rows_to_first<VEC, 2>(lds, me.rows, s.slab, me.row, me.col, me.active, sum);
+  if (me.active && me.row == 0)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float *o = sums + (((long long)n * s.chunks + chunk_index) * s.C + c0 + e) * 2;
+      o[0] = sum[0][e];
+      o[1] = sum[1][e];
+    }
+}
+
+// One workgroup per (image, group): the chunks' sums become E d and E (d xhat), and the image's per-channel sums.
+__global__ __launch_bounds__(256) void norm_grad_join_kernel(const float *__restrict__ sums, const float *__restrict__ gamma,
+                                                             float *__restrict__ image_sums, float *__restrict__ expect, NormShape s) {
+  const int g = (int)(blockIdx.x % (unsigned)s.G), n = (int)(blockIdx.x / (unsigned)s.G);
+  __shared__ float red[2][4];
+  float d1 = 0.0f, d2 = 0.0f;
+  for (int c = threadIdx.x; c < s.Cg; c += 256) {
+    const int ch = g * s.Cg + c;
+    float a = 0.0f, b = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < s.chunks; ++k) {
+      const f32x2 v = *reinterpret_cast<const f32x2 *>(sums + (((long long)n * s.chunks + k) * s.C + ch) * 2);
+      a += v.x;
+      b += v.y;
+    }
+    *reinterpret_cast<f32x2 *>(image_sums + ((long long)n * s.C + ch) * 2) = f32x2{a, b};
+    d1 = __builtin_fmaf(a, gamma[ch], d1);
+    d2 = __builtin_fmaf(b, gamma[ch], d2);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    d1 += __shfl_xor(d1, d);
+    d2 += __shfl_xor(d2, d);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = d1;
+    red[1][threadIdx.x >> 6] = d2;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    const float *r = red[threadIdx.x];
+    expect[((long long)n * s.G + g) * 2 + threadIdx.x] = (r[0] + r[1] + (r[2] + r[3])) / ((float)s.S * (float)s.Cg);
+  }
+}
+
+template <typename T, int VEC, int NT>
+__global__ __launch_bounds__(NT) void norm_grad_apply_kernel(const T *__restrict__ dy, const T *__restrict__ x,
+                                                             const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                             const float *__restrict__ stats, const float *__restrict__ expect,
+                                                             T *__restrict__ dx, NormShape s, int act) {
+  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
+  const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
+  const int chunk_index = rest % s.chunks, n = rest / s.chunks;
+  const Column<T, VEC, NT> me(s, slab_index);
+  if (!me.active) return;
+  const int c0 = slab_index * s.slab + me.col;
+  const int p0 = chunk_index * s.chunk;
+  const int count = min(s.chunk, s.S - p0);
+  const long long base = ((long long)n * s.S + p0) * s.C + c0;
+  GradCoefficients<VEC> k;
+  k.load(stats, gamma, beta, s, n, c0);
+  float d1[VEC], d2[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const float *o = expect + ((long long)n * s.G + (c0 + e) / s.Cg) * 2;
+    d1[e] = o[0];
+    d2[e] = o[1];
+  }
+#pragma unroll 4
+  for (int p = me.row; p < count; p += me.rows) {
+    float fx[VEC], fd[VEC];
+    Pack<T, VEC>::load(x + base + (long long)p * s.C).unpack(fx);
+    Pack<T, VEC>::load(dy + base + (long long)p * s.C).unpack(fd);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float xhat, dz;
+      k.of(e, fx[e], fd[e], act, xhat, dz);
+      fd[e] = k.rstd[e] * (__builtin_fmaf(dz, k.gamma[e], -d1[e]) - xhat * d2[e]);
+    }
+    Pack<T, VEC>::store(dx + base + (long long)p * s.C, fd);
+  }
+}
+
+// dbeta[c], dgamma[c] = the sums of `parts` rows of (C, 2): 8 channels per workgroup, 64 threads down the rows of each.
+__global__ __launch_bounds__(1024) void norm_grad_params_kernel(const float *__restrict__ sums, long long parts, int C,
+                                                                float *__restrict__ dgamma, float *__restrict__ dbeta) {
+  __shared__ float red[64][17];
+  const int j = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const long long at = (long long)blockIdx.x * 16 + j;  // of 2 C
+  float s = 0.0f;
+  if (at < 2ll * C) {
+#pragma unroll 8
+    for (long long p = r; p < parts; p += 64) s += sums[p * 2 * C + at];
+  }
+  red[r][j] = s;
+  __syncthreads();
+  for (int half = 32; half > 0; half >>= 1) {
+    if (r < half) red[r][j] += red[r + half][j];
+    __syncthreads();
+  }
+  if (r == 0 && at < 2ll * C) ((at & 1) ? dgamma : dbeta)[at >> 1] = red[0][j];
+}
+
+// ---- the choice of a split -------------------------------------------------------------------------------------------------
+static const int kNormThreads = 512;
+static const int kNormMaxColumns = kNormThreads;  // packs of a slab: at least one row of threads
+static const int kNormTargetGroups = 1024;        // workgroups that fill the chip twice over at two per CU
+
+struct NormPlan {
+  NormShape s;
+  int vec;    // elements per pack; 0: not supported
+  int nv;     // packs a thread holds: 1, 2, 4, 8 (forward: 16)
+  bool resident;
+  int rows;   // rows of threads
+};
+
+static int gcd_int(int a, int b) { return b ? gcd_int(b, a % b) : a; }
+
+// Whole image per workgroup where a slab's packs fit `most` per thread, chunks of positions otherwise.
+static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, int most) {
+  NormPlan p = {};
+  p.s.N = N, p.s.S = S, p.s.C = C, p.s.G = G, p.s.Cg = C / G;
+  int vec = aligned && ((long long)C * elem) % 16 == 0 ? 16 / elem : 1;
+  long long unit = (long long)p.s.Cg / gcd_int(p.s.Cg, vec) * vec;  // channels: whole groups and whole packs
+  if (unit / vec > kNormMaxColumns && vec > 1) {
+    vec = 1;
+    unit = p.s.Cg;
+  }
+  if (unit / vec > kNormMaxColumns) return p;
+  p.vec = vec;
+  const long long units = C / unit;
+  long long k = kNormMaxColumns * (long long)vec / unit;  // units per slab
+  if (k > units) k = units;
+  auto fits = [&](long long kk) { return (S + kNormThreads / (int)(kk * unit / vec) - 1) / (kNormThreads / (int)(kk * unit / vec)) <= most; };
+  auto groups = [&](long long kk) { return (long long)N * ((units + kk - 1) / kk); };
+  while (k > 1 && !fits(k)) k = (k + 1) / 2;
+  p.resident = fits(k);
+  if (p.resident) {
+    // narrower slabs while the chip is not full and a slab's row is still a full 128-byte line
+    while (k > 1 && groups(k) < kNormTargetGroups && (k + 1) / 2 * unit * elem >= 128) k = (k + 1) / 2;
+    p.s.chunk = S;
+    p.s.chunks = 1;
+  } else {
+    k = kNormMaxColumns * (long long)vec / unit;
+    if (k > units) k = units;
+  }
+  p.s.slab = (int)(k * unit);
+  p.s.slabs = (int)((units + k - 1) / k);
+  p.rows = kNormThreads / (p.s.slab / vec);
+  if (!p.resident) {
+    int per = most;  // passes per chunk: as many as fit, fewer while the chip is not full
+    while (per > 2 && (long long)N * p.s.slabs * ((S + p.rows * per - 1) / (p.rows * per)) < kNormTargetGroups) per /= 2;
+    p.s.chunk = p.rows * per;
+    p.s.chunks = (S + p.s.chunk - 1) / p.s.chunk;
+  }
+  const int need = (p.s.chunk + p.rows - 1) / p.rows;
+  p.nv = 1;
+  while (p.nv < need) p.nv *= 2;
+  return p;
+}
+
+static const int kNormForwardMost = 16, kNormGradMost = 8;
+
+static int grad_images_per_group(const NormPlan &p) {
+  const long long per = ((long long)p.s.N * p.s.slabs + 4095) / 4096;
+  return (int)per;
+}
+
+template <typename T, int VEC>
+static int launch_norm(const NormPlan &p, const void *x, void *y, const float *gamma, const float *beta, float *stats,
+                       float *workspace, float eps, int act, hipStream_t stream) {
+  constexpr int NT = kNormThreads;
+  const size_t lds = ((size_t)p.rows * p.s.slab + 2 * (p.s.slab / p.s.Cg)) * sizeof(float);
+  const dim3 grid((unsigned)((long long)p.s.N * p.s.chunks * p.s.slabs));
+  float *out = p.resident ? stats : workspace;
+#define FRCNN_NORM(NV, W)                                                                                                   \
+  {                                                                                                                         \
+    const int rc = ensure_dynamic_lds((const void *)norm_resident_kernel<T, VEC, NV, NT, W>, lds, "group_norm");            \
+    if (rc) return rc;                                                                                                      \
+    hipLaunchKernelGGL((norm_resident_kernel<T, VEC, NV, NT, W>), grid, dim3(NT), lds, stream, (const T *)x, (T *)y, gamma, \
+                       beta, out, p.s, eps, act);                                                                           \
+  }
+  if (p.resident) {
+    if (p.nv == 1) FRCNN_NORM(1, true) else if (p.nv == 2) FRCNN_NORM(2, true) else if (p.nv == 4) FRCNN_NORM(4, true)
+    else if (p.nv == 8) FRCNN_NORM(8, true) else FRCNN_NORM(16, true)
+    return check_launch("group_norm");
+  }
+  if (p.nv <= 2) FRCNN_NORM(2, false) else if (p.nv == 4) FRCNN_NORM(4, false) else if (p.nv == 8) FRCNN_NORM(8, false)
+  else FRCNN_NORM(16, false)
+#undef FRCNN_NORM
+  int rc = check_launch("group_norm");
+  if (rc) return rc;
+  float *joined = stats ? stats : workspace + (size_t)p.s.N * p.s.chunks * p.s.G * 2;
+  hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(((long long)p.s.N * p.s.G + 3) / 4)), dim3(256), 0, stream, workspace,
+                     joined, p.s, eps);
+  rc = check_launch("group_norm");
+  if (rc) return rc;
+  hipLaunchKernelGGL((norm_apply_kernel<T, VEC, NT>), grid, dim3(NT), 0, stream, (const T *)x, (T *)y, gamma, beta, joined, p.s,
+                     act);
+  return check_launch("group_norm");
+}
+
+template <typename T, int VEC>
+static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, const float *gamma, const float *beta,
+                            const float *stats, void *dx, float *dgamma, float *dbeta, float *workspace, int act,
+                            hipStream_t stream) {
+  constexpr int NT = kNormThreads;
+  const NormShape &s = p.s;
+  long long parts;
+  float *sums = workspace;
+  int rc;
+  if (p.resident) {
+    const int per = grad_images_per_group(p);
+    parts = (s.N + per - 1) / per;
+    const size_t lds = (2 * (size_t)p.rows * s.slab + 2 * (s.slab / s.Cg) + s.slab) * sizeof(float);
+    const dim3 grid((unsigned)(parts * s.slabs));
+#define FRCNN_NORM_GRAD(NV)                                                                                                    \
+  {                                                                                                                            \
+    rc = ensure_dynamic_lds((const void *)norm_grad_resident_kernel<T, VEC, NV, NT>, lds, "group_norm_grad");                  \
+    if (rc) return rc;                                                                                                         \
+    hipLaunchKernelGGL((norm_grad_resident_kernel<T, VEC, NV, NT>), grid, dim3(NT), lds, stream, (const T *)dy, (const T *)x,  \
+                       gamma, beta, stats, (T *)dx, sums, s, per, act);                                                        \
+  }
+    if (p.nv == 1) FRCNN_NORM_GRAD(1) else if (p.nv == 2) FRCNN_NORM_GRAD(2) else if (p.nv == 4) FRCNN_NORM_GRAD(4)
+    else FRCNN_NORM_GRAD(8)
+#undef FRCNN_NORM_GRAD
+    rc = check_launch("group_norm_grad");
+    if (rc) return rc;
+  } else {
+    parts = s.N;
+    float *expect = workspace, *image_sums = expect + (size_t)s.N * s.G * 2;
+    float *chunk_sums = image_sums + (size_t)s.N * s.C * 2;
+    sums = image_sums;
+    const dim3 grid((unsigned)((long long)s.N * s.chunks * s.slabs));
+    const size_t lds = 2 * (size_t)p.rows * s.slab * sizeof(float);
+    rc = ensure_dynamic_lds((const void *)norm_grad_sums_kernel<T, VEC, NT>, lds, "group_norm_grad");
+    if (rc) return rc;
+    hipLaunchKernelGGL((norm_grad_sums_kernel<T, VEC, NT>), grid, dim3(NT), lds, stream, (const T *)dy, (const T *)x, gamma, beta,
+                       stats, chunk_sums, s, act);
+    rc = check_launch("group_norm_grad");
+    if (rc) return rc;
+    hipLaunchKernelGGL(norm_grad_join_kernel, dim3((unsigned)(s.N * s.G)), dim3(256), 0, stream, chunk_sums, gamma, image_sums,
+                       expect, s);
+    rc = check_launch("group_norm_grad");
+    if (rc) return rc;
+    hipLaunchKernelGGL((norm_grad_apply_kernel<T, VEC, NT>), grid, dim3(NT), 0, stream, (const T *)dy, (const T *)x, gamma, beta,
+                       stats, expect, (T *)dx, s, act);
+    rc = check_launch("group_norm_grad");
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL(norm_grad_params_kernel, dim3((unsigned)((2ll * s.C + 15) / 16)), dim3(1024), 0, stream, sums, parts, s.C,
+                     dgamma, dbeta);
+  return check_launch("group_norm_grad");
+}
+
+// What the two entry points ask of a shape.
+static int norm_check(const char *what, int type, int64_t N, int64_t S, int C, int G, int act) {
+  FRCNN_REQUIRE(type_known(type), "%s: unknown element type %d", what, type);
+  FRCNN_REQUIRE(N >= 0 && S >= 1, "%s: needs at least one position per image (N=%lld, S=%lld)", what, (long long)N, (long long)S);
+  FRCNN_REQUIRE(C >= 1 && G >= 1 && C % G == 0, "%s: %d channels are not a multiple of %d groups", what, C, G);
+  FRCNN_REQUIRE(act == FRCNN_ACT_NONE || act == FRCNN_ACT_RELU || act == FRCNN_ACT_SWISH, "%s: unknown activation %d", what, act);
+  if (N >= (1ll << 31) || S >= (1ll << 24) || C > (1 << 20) || N * G >= (1ll << 31) || N * C >= (1ll << 38))
+    return set_error(FRCNN_EUNSUPPORTED, "%s: (%lld, %lld, %d) is beyond what the kernels index", what, (long long)N, (long long)S, C);
+  return FRCNN_OK;
+}
+
+// The plan may depend on the pointers' alignment only through `vec`; workspaces are sized for the larger of the two.
+static size_t norm_bytes(int N, int S, int C, int G, int elem, bool grad) {
+  size_t most = 0;
+  for (int aligned = 0; aligned < 2; ++aligned) {
+    const NormPlan p = norm_plan(N, S, C, G, elem, aligned != 0, grad ? kNormGradMost : kNormForwardMost);
+    if (!p.vec) continue;
+    size_t floats;
+    if (!grad) {
+      floats = p.resident ? 0 : (size_t)N * (p.s.chunks + 1) * G * 2;
+    } else if (p.resident) {
+      const int per = grad_images_per_group(p);
+      floats = (size_t)((N + per - 1) / per) * C * 2;
+    } else {
+      floats = (size_t)N * G * 2 + (size_t)N * C * 2 + (size_t)N * p.s.chunks * C * 2;
+    }
+    if (floats > most) most = floats;
+  }
+  return most * sizeof(float);
+}
+
+}  // namespace frcnn
+
+using namespace frcnn;
+
+extern "C" {
+
+size_t frcnn_group_norm_workspace_bytes(int type, int64_t N, int64_t S, int C, int G) {
+  if (norm_check("group_norm", type, N, S, C, G, FRCNN_ACT_NONE) || N == 0) return 0;
+  return norm_bytes((int)N, (int)S, C, G, (int)type_bytes(type), false);
+}
+
+int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int C, int G, const float *gamma, const float *beta,
+                     float epsilon, int activation, void *y, float *stats, void *workspace, size_t workspace_bytes,
+                     frcnn_stream_t stream) {
+  const int bad = norm_check("group_norm", type, N, S, C, G, activation);
+  if (bad) return bad;
+  FRCNN_REQUIRE(epsilon >= 0.0f, "group_norm: epsilon %g is negative", (double)epsilon);
+  if (N == 0) return FRCNN_OK;
+  FRCNN_REQUIRE(x && gamma && beta && y, "group_norm: null pointer");
+  const int elem = (int)type_bytes(type);
+  FRCNN_REQUIRE(aligned_to(x, elem) && aligned_to(y, elem) && aligned_to(gamma, 4) && aligned_to(beta, 4) && aligned_to(stats, 4),
+                "group_norm: misaligned pointer");
+  const NormPlan p = norm_plan((int)N, (int)S, C, G, elem, aligned_to(x, 16) && aligned_to(y, 16), kNormForwardMost);
+  if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm: %d channels per group", C / G);
+  if ((long long)N * p.s.chunks * p.s.slabs >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "group_norm: too many workgroups");
+  const size_t need = frcnn_group_norm_workspace_bytes(type, N, S, C, G);
+  FRCNN_REQUIRE(need == 0 || (workspace && aligned_to(workspace, 256) && workspace_bytes >= need),
+                "group_norm: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  float *ws = (float *)workspace;
+#define FRCNN_NORM_T(T)                                                                                       \
+  (p.vec > 1 ? launch_norm<T, 16 / sizeof(T)>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st)       \
+             : launch_norm<T, 1>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st))
+  if (type == FRCNN_F32) return FRCNN_NORM_T(float);
+  if (type == FRCNN_F16) return FRCNN_NORM_T(_Float16);
+  return FRCNN_NORM_T(__bf16);
+#undef FRCNN_NORM_T
+}
+
+size_t frcnn_group_norm_grad_workspace_bytes(int type, int64_t N, int64_t S, int C, int G) {
+  if (norm_check("group_norm_grad", type, N, S, C, G, FRCNN_ACT_NONE) || N == 0) return 0;
+  return norm_bytes((int)N, (int)S, C, G, (int)type_bytes(type), true);
+}
+
+int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, int64_t S, int C, int G, const float *gamma,
+                          const float *beta, const float *stats, int activation, void *dx, float *dgamma, float *dbeta,
+                          void *workspace, size_t workspace_bytes, frcnn_stream_t stream) {
+  const int bad = norm_check("group_norm_grad", type, N, S, C, G, activation);
+  if (bad) return bad;
+  FRCNN_REQUIRE(dgamma && dbeta, "group_norm_grad: null pointer");
+  FRCNN_REQUIRE(aligned_to(dgamma, 4) && aligned_to(dbeta, 4), "group_norm_grad: misaligned pointer");
+  hipStream_t st = (hipStream_t)stream;
+  if (N == 0) {  // sums over nothing
+    hipLaunchKernelGGL(norm_grad_params_kernel, dim3((unsigned)((2ll * C + 15) / 16)), dim3(1024), 0, st, (const float *)nullptr, 0ll,
+                       C, dgamma, dbeta);
+    return check_launch("group_norm_grad");
+  }
+  FRCNN_REQUIRE(dy && x && gamma && beta && stats && dx, "group_norm_grad: null pointer");
+  const int elem = (int)type_bytes(type);
+  FRCNN_REQUIRE(aligned_to(dy, elem) && aligned_to(x, elem) && aligned_to(dx, elem) && aligned_to(gamma, 4) && aligned_to(beta, 4) &&
+                    aligned_to(stats, 4),
+                "group_norm_grad: misaligned pointer");
+  const NormPlan p = norm_plan((int)N, (int)S, C, G, elem, aligned_to(x, 16) && aligned_to(dy, 16) && aligned_to(dx, 16), kNormGradMost);
+  if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: %d channels per group", C / G);
+  if ((long long)N * p.s.chunks * p.s.slabs >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: too many workgroups");
+  const size_t need = frcnn_group_norm_grad_workspace_bytes(type, N, S, C, G);
+  FRCNN_REQUIRE(workspace && aligned_to(workspace, 256) && workspace_bytes >= need,
+                "group_norm_grad: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);
+  float *ws = (float *)workspace;
+#define FRCNN_NORM_T(T)                                                                                                        \
+  (p.vec > 1 ? launch_norm_grad<T, 16 / sizeof(T)>(p, dy, x, gamma, beta, stats, dx, dgamma, dbeta, ws, activation, st)        \
+             : launch_norm_grad<T, 1>(p, dy, x, gamma, beta, stats, dx, dgamma, dbeta, ws, activation, st))
+  if (type == FRCNN_F32) return FRCNN_NORM_T(float);
+  if (type == FRCNN_F16) return FRCNN_NORM_T(_Float16);
+  return FRCNN_NORM_T(__bf16);
+#undef FRCNN_NORM_T
+}
+
+}  // extern "C"
