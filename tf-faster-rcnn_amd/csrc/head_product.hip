@@ -30,10 +30,13 @@ struct ProductArgs {
 // The 16 bytes at `col` of a row of K bytes; bytes at K and beyond are zero.
 __device__ __forceinline__ u32x4 load_chunk(const uint8_t *row, int col, int K) {
   if (col + 16 <= K) return *reinterpret_cast<const u32x4 *>(row + col);
-  u32x4 w = {0, 0, 0, 0};
-  for (int i = 0; i < 16; ++i)
-    if (col + i < K) w[i >> 2] |= (uint32_t)row[col + i] << (8 * (i & 3));
-  return w;
+  uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+  for (int i = K - col - 1; i >= 0; --i) {
+    hi = hi << 8 | lo >> 56;
+    lo = lo << 8 | row[col + i];
+  }
+  return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
 
 // Lane l of an operand holds row l % 16 and, of the block's eight 16-byte chunks, number l / 16 and l / 16 + 4 (both operands
@@ -195,6 +198,198 @@ __global__ __launch_bounds__(64 * W) void product_split_kernel(ProductArgs p, in
   }
 }
 
+// ---- large products: tiles through LDS ------------------------------------------------------------------------------------------
+// A workgroup of WM x WN waves computes a BM x BN tile, 16 MT x 16 NT per wave, one block of 128 columns at a time: the next
+// block travels from memory straight to the other half of LDS while the matrix instructions work on this one.  In LDS a row of
+// 128 bytes keeps its 16-byte chunk c at place c ^ (row % 8), so that the 16 rows of an operand read fall on all banks.
+//
+// The tiles fill the chip in rounds of one workgroup per CU; the tiles of a last, unfilled round are cut along K into `pieces`
+// of whole blocks, whose sums go to the workspace and are added in their order by product_join_kernel.
+static const int kProductCus = 256;
+
+struct TilePlan {
+  int tiles_m, tiles_n;
+  int whole;   // tiles computed by one workgroup each: the first ones of the order
+  int rest;    // the others
+  int pieces;  // workgroups per tile of the rest
+};
+
+static const int kStripRows = 4;
+
+// Workgroups are dealt to the 8 XCDs in turn: give each a contiguous range of the order, which runs down strips of kStripRows
+// row tiles, so that the 32 tiles an XCD works on share 4 rows' and 8 columns' operands in its L2.
+__device__ __forceinline__ int xcd_contiguous(int i, int n) {
+  const int x = i & 7, base = n >> 3, more = n & 7;
+  return x * base + min(x, more) + (i >> 3);
+}
+
+__device__ __forceinline__ void tile_of(const TilePlan &t, int order, int &m, int &n) {
+  const int strip = order / (kStripRows * t.tiles_n), at = order - strip * kStripRows * t.tiles_n;
+  const int rows = min(kStripRows, t.tiles_m - strip * kStripRows);
+  n = at / rows;
+  m = strip * kStripRows + at - n * rows;
+}
+
+typedef __attribute__((address_space(1))) const void *global_ptr;
+typedef __attribute__((address_space(3))) void *lds_ptr;
+
+// The R rows of one operand's tile, a block at a time, into LDS.
+template <int R, int THREADS>
+struct TileLoader {
+  static constexpr int N = R * 8 / THREADS;  // 16-byte chunks per thread
+  static_assert(R * 8 % THREADS == 0, "whole rounds of chunks");
+  const uint8_t *base;  // the tile's first row
+  unsigned offset[N];
+  int first, rows, ld;
+  __device__ __forceinline__ TileLoader(const uint8_t *operand, long long stride, int first_row, int total_rows)
+      : base(operand + first_row * stride), first(first_row), rows(total_rows), ld((int)stride) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = i * THREADS + (int)threadIdx.x, row = c >> 3;
+      offset[i] = (unsigned)(min(row, rows - 1 - first) * ld + (((c & 7) ^ (row & 7)) << 4));  // rows beyond the end: the last one
+    }
+  }
+  __device__ __forceinline__ void start(int block, uint8_t *lds) const {
+    const uint8_t *p = base + (long long)block * kQuantBlock;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      __builtin_amdgcn_global_load_lds((global_ptr)(p + offset[i]), (lds_ptr)(lds + (i * THREADS + wave * 64) * 16), 16, 0, 0);
+  }
+  // the last, partial block: zeros behind the row's end
+  __device__ __forceinline__ void partial(int block, int K, uint8_t *lds) const {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {
+      const int c = i * THREADS + (int)threadIdx.x, row = c >> 3;
+      const uint8_t *r = base + (long long)min(row, rows - 1 - first) * ld;
+      *reinterpret_cast<u32x4 *>(lds + c * 16) = load_chunk(r, block * kQuantBlock + ((c & 7) ^ (row & 7)) * 16, K);
+    }
+  }
+};
+
+// `at`: the first of the lane's two chunks in row lane % 16 of the operand's tile; rows further down are 2 KB per 16 apart.
+__device__ __forceinline__ i32x8 read_operand(const uint8_t *lds, int at, int sixteens) {
+  const u32x4 lo = *reinterpret_cast<const u32x4 *>(lds + at + sixteens * (16 * kQuantBlock));
+  const u32x4 hi = *reinterpret_cast<const u32x4 *>(lds + (at ^ 64) + sixteens * (16 * kQuantBlock));
+  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+
+template <int MT, int NT, int WM, int WN, int MODE>
+__global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs p, TilePlan plan, f32x4 *__restrict__ partial) {
+  constexpr int THREADS = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
+  constexpr int HALF = (BM + BN) * kQuantBlock + BM * 4;  // a's tile, b's tile, a's scales
+  static_assert(BM <= THREADS, "a thread per row loads a scale");
+  using S = Scale<MODE>;
+  using O = Operand<MODE>;
+  extern __shared__ uint8_t smem[];
+  int tile, k0 = 0, k1 = p.blocks, piece = -1;
+  if ((int)blockIdx.x < plan.whole) {
+    tile = xcd_contiguous((int)blockIdx.x, plan.whole);
+  } else {  // the same blocks of K of neighbouring tiles next to each other
+    const int r = xcd_contiguous((int)blockIdx.x - plan.whole, plan.rest * plan.pieces);
+    const int part = r / plan.rest, t = r - part * plan.rest;
+    tile = plan.whole + t;
+    k0 = __builtin_amdgcn_readfirstlane((int)((long long)p.blocks * part / plan.pieces));
+    k1 = __builtin_amdgcn_readfirstlane((int)((long long)p.blocks * (part + 1) / plan.pieces));
+    if (plan.pieces > 1) piece = t * plan.pieces + part;
+  }
+  int tm, tn;
+  tile_of(plan, tile, tm, tn);
+  const int m0 = __builtin_amdgcn_readfirstlane(tm) * BM, n0 = __builtin_amdgcn_readfirstlane(tn) * BN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
+  const int wm = (wave % WM) * MT * 16, wn = (wave / WM) * NT * 16;  // the wave's corner in the tile
+  const TileLoader<BM, THREADS> load_a(p.a, p.lda, m0, p.M);
+  const TileLoader<BN, THREADS> load_b(p.b, p.ldb, n0, p.N);
+  const int whole_blocks = p.K / kQuantBlock;
+  // NT * 16 divides 128: one row of b's scales
+  const long long sb_at = (long long)(min(n0 + wn, p.N - 1) / kQuantBlock) * p.sb_row;
+  const long long sa_at = (long long)min(m0 + (int)threadIdx.x, p.M - 1) * p.sa_row;
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  typename S::type sa_next = 0, sb_next = 0;
+  auto fetch = [&](int block, uint8_t *to) {
+    if (block < whole_blocks) {
+      load_a.start(block, to);
+      load_b.start(block, to + BM * kQuantBlock);
+    } else {
+      load_a.partial(block, p.K, to);
+      load_b.partial(block, p.K, to + BM * kQuantBlock);
+    }
+    if (BM == THREADS || threadIdx.x < BM) sa_next = S::load(p.sa, sa_at + block * p.sa_block);
+    sb_next = S::load(p.sb, sb_at + block * p.sb_block);
+  };
+  const int lane_at = (lane & 15) * kQuantBlock + (((lane >> 4) ^ (lane & 7)) << 4);
+  if (k0 < k1) fetch(k0, smem);
+  for (int kb = k0; kb < k1; ++kb) {
+    uint8_t *half = smem + ((kb - k0) & 1) * HALF;
+    typename S::type *scales = reinterpret_cast<typename S::type *>(half + (BM + BN) * kQuantBlock);
+    if (BM == THREADS || threadIdx.x < BM) scales[threadIdx.x] = sa_next;
+    const typename S::type sb = sb_next;
+    // this block has arrived, and every wave is done with the other half
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (kb + 1 < k1) fetch(kb + 1, smem + ((kb + 1 - k0) & 1) * HALF);
+    const uint8_t *a = half + wm * kQuantBlock, *b = half + (BM + wn) * kQuantBlock;
+    typename O::type w[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w[j] = O::of(read_operand(b, lane_at, j));
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const typename O::type x = O::of(read_operand(a, lane_at, i));
+      const typename S::type sa = scales[wm + i * 16 + (lane & 15)];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = multiply<MODE>(w[j], x, acc[i][j], sb, sa);
+    }
+  }
+  if (piece >= 0) {
+    f32x4 *out = partial + (long long)piece * (MT * NT * THREADS) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) out[(i * NT + j) * THREADS] = acc[i][j];
+  } else {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) finish4(p, m0 + wm + i * 16 + (lane & 15), n0 + wn + j * 16 + (lane >> 4) * 4, acc[i][j]);
+  }
+}
+
+// One workgroup per 16 x 16 tile index of a cut tile's waves: the pieces' sums in their order, then what a whole tile does.
+template <int MT, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void product_join_kernel(ProductArgs p, TilePlan plan, const f32x4 *__restrict__ partial) {
+  constexpr int THREADS = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
+  const int t = (int)(blockIdx.x / (MT * NT)), f = (int)(blockIdx.x % (MT * NT));
+  int tm, tn;
+  tile_of(plan, plan.whole + t, tm, tn);
+  const int wave = threadIdx.x >> 6, lane = lane_id();
+  const int m = tm * BM + (wave % WM) * MT * 16 + (f / NT) * 16 + (lane & 15);
+  const int n = tn * BN + (wave / WM) * NT * 16 + (f % NT) * 16 + (lane >> 4) * 4;
+  const f32x4 *in = partial + ((long long)t * plan.pieces * (MT * NT) + f) * THREADS + threadIdx.x;
+  f32x4 v = in[0];
+#pragma unroll 4
+  for (int i = 1; i < plan.pieces; ++i) v += in[(long long)i * (MT * NT * THREADS)];
+  finish4(p, m, n, v);
+}
+
+static TilePlan tile_plan(int M, int N, int blocks, int bm, int bn) {
+  TilePlan t;
+  t.tiles_m = (M + bm - 1) / bm;
+  t.tiles_n = (N + bn - 1) / bn;
+  const long long tiles = (long long)t.tiles_m * t.tiles_n;
+  t.whole = (int)(tiles / kProductCus * kProductCus);
+  t.rest = (int)(tiles - t.whole);
+  t.pieces = t.rest ? kProductCus / t.rest : 1;
+  if (t.pieces > blocks / 4) t.pieces = blocks / 4;  // at least four blocks each: the first one's latency is not hidden
+  if (t.pieces < 1) t.pieces = 1;
+  return t;
+}
+
 }  // namespace frcnn
 
 using namespace frcnn;
@@ -202,8 +397,9 @@ using namespace frcnn;
 extern "C" {
 
 size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K) {
-  (void)M, (void)N, (void)K;
-  return 0;
+  if (M < 200 || N < 200 || K < 0) return 0;
+  const TilePlan t = tile_plan(M, N, (K + kQuantBlock - 1) / kQuantBlock, 256, 256);
+  return t.pieces > 1 ? (size_t)t.rest * t.pieces * 256 * 256 * sizeof(float) : 0;
 }
 
 int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_scale_row_stride, int64_t a_scale_block_stride,
@@ -228,7 +424,9 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
   if (K > (1 << 22) || lda > (1 << 23) || ldb > (1 << 23) || N > (1 << 24))
     return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: K=%d (row strides %lld, %lld), N=%d is beyond what the kernels index", K,
                      (long long)lda, (long long)ldb, N);
-  (void)workspace, (void)workspace_bytes;
+  const size_t need = frcnn_scaled_matmul_workspace_bytes(M, N, K);
+  FRCNN_REQUIRE(need == 0 || (workspace && aligned_to(workspace, 256) && workspace_bytes >= need),
+                "scaled_matmul: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);
   const ProductArgs p = {(const uint8_t *)a, (const uint8_t *)b, lda, ldb, a_scales, b_scales, a_scale_row_stride, a_scale_block_stride,
                          b_scale_row_stride, b_scale_block_stride, bias, y, ldy, M, N, K, (K + kQuantBlock - 1) / kQuantBlock,
                          activation, y_type};
@@ -244,8 +442,34 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
     else if (mode == kWideF32) hipLaunchKernelGGL((product_split_kernel<TM, TN, W, kWideF32>), grid, block, 0, s, p, (int)tn); \
     else hipLaunchKernelGGL((product_split_kernel<TM, TN, W, kWideE8M0>), grid, block, 0, s, p, (int)tn);                      \
   }
-  if (M <= 16) FRCNN_SPLIT(1, 1, 16) else FRCNN_SPLIT(4, 2, 4)
+#define FRCNN_TILE_MODE(MT, NT, WM, WN, MODE)                                                                                   \
+  {                                                                                                                             \
+    const int rc = ensure_dynamic_lds((const void *)product_tile_kernel<MT, NT, WM, WN, MODE>, lds, "scaled_matmul");           \
+    if (rc) return rc;                                                                                                          \
+    hipLaunchKernelGGL((product_tile_kernel<MT, NT, WM, WN, MODE>), grid, dim3(64 * WM * WN), lds, s, p, plan, (f32x4 *)workspace); \
+  }
+#define FRCNN_TILE(MT, NT, WM, WN)                                                                                              \
+  {                                                                                                                             \
+    const TilePlan plan = tile_plan(M, N, p.blocks, 16 * MT * WM, 16 * NT * WN);                                                \
+    const size_t lds = 2 * ((16 * MT * WM + 16 * NT * WN) * kQuantBlock + 64 * MT * WM);                                                   \
+    const dim3 grid((unsigned)(plan.whole + plan.rest * plan.pieces));                                                          \
+    if (mode == kNarrowF32) FRCNN_TILE_MODE(MT, NT, WM, WN, kNarrowF32)                                                         \
+    else if (mode == kNarrowE8M0) FRCNN_TILE_MODE(MT, NT, WM, WN, kNarrowE8M0)                                                  \
+    else if (mode == kWideF32) FRCNN_TILE_MODE(MT, NT, WM, WN, kWideF32)                                                        \
+    else FRCNN_TILE_MODE(MT, NT, WM, WN, kWideE8M0)                                                                             \
+    if (plan.pieces > 1) {                                                                                                      \
+      const int rc = check_launch("scaled_matmul");                                                                             \
+      if (rc) return rc;                                                                                                        \
+      hipLaunchKernelGGL((product_join_kernel<MT, NT, WM, WN>), dim3((unsigned)(plan.rest * MT * NT)), dim3(64 * WM * WN), 0, s, p, plan, \
+                         (const f32x4 *)workspace);                                                                             \
+    }                                                                                                                           \
+  }
+  if (M <= 16) FRCNN_SPLIT(1, 1, 16)
+  else if (M < 200 || N < 200) FRCNN_SPLIT(4, 2, 4)
+  else FRCNN_TILE(8, 4, 2, 4)
 #undef FRCNN_SPLIT
+#undef FRCNN_TILE
+#undef FRCNN_TILE_MODE
   return check_launch("scaled_matmul");
 }
 
