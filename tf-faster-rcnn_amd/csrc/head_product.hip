@@ -99,24 +99,33 @@ struct Operand<kWideF32> {
 template <>
 struct Operand<kWideE8M0> : Operand<kWideF32> {};
 
+// The 128 products of a block onto acc: with its scales only where the instruction takes them.
 template <int MODE>
-__device__ __forceinline__ f32x4 multiply(const typename Operand<MODE>::type &w, const typename Operand<MODE>::type &a, f32x4 acc,
-                                          typename Scale<MODE>::type sw, typename Scale<MODE>::type sa) {
+__device__ __forceinline__ f32x4 block_product(const typename Operand<MODE>::type &w, const typename Operand<MODE>::type &a, f32x4 acc,
+                                               typename Scale<MODE>::type sw, typename Scale<MODE>::type sa) {
   if constexpr (MODE == kNarrowE8M0) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, sw, 0, sa);
+  } else if constexpr (MODE == kNarrowF32) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, 0, 0, 0);
   } else {
-    f32x4 d = {0, 0, 0, 0};
-    if constexpr (MODE == kNarrowF32) {
-      d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, d, 0, 0, 0, 0, 0, 0);
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[i], a.h[i], d, 0, 0, 0);
-    }
-    const float s = sw * sa;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
+    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[i], a.h[i], acc, 0, 0, 0);
     return acc;
   }
+}
+
+__device__ __forceinline__ void add_scaled(f32x4 &acc, f32x4 d, float s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
+}
+
+template <int MODE>
+__device__ __forceinline__ void multiply(const typename Operand<MODE>::type &w, const typename Operand<MODE>::type &a, f32x4 &acc,
+                                         typename Scale<MODE>::type sw, typename Scale<MODE>::type sa) {
+  if constexpr (MODE == kNarrowE8M0)
+    acc = block_product<MODE>(w, a, acc, sw, sa);
+  else
+    add_scaled(acc, block_product<MODE>(w, a, f32x4{0, 0, 0, 0}, sw, sa), sw * sa);
 }
 
 // Bias, activation, rounding and store of four neighbouring columns n .. n + 3 of row m.
@@ -182,7 +191,7 @@ __global__ __launch_bounds__(64 * W) void product_split_kernel(ProductArgs p, in
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = multiply<MODE>(b[j], a[i], acc[i][j], sb[j], sa[i]);
+      for (int j = 0; j < TN; ++j) multiply<MODE>(b[j], a[i], acc[i][j], sb[j], sa[i]);
   }
   __shared__ f32x4 part[W][TM * TN][64];
 #pragma unroll
@@ -200,7 +209,7 @@ __global__ __launch_bounds__(64 * W) void product_split_kernel(ProductArgs p, in
 
 // ---- large products: tiles through LDS ------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves computes a BM x BN tile, 16 MT x 16 NT per wave, one block of 128 columns at a time: the next
-// block travels from memory straight to the other half of LDS while the matrix instructions work on this one.  In LDS a row of
+// blocks travel from memory straight to other parts of LDS while the matrix instructions work on this one.  In LDS a row of
 // 128 bytes keeps its 16-byte chunk c at place c ^ (row % 8), so that the 16 rows of an operand read fall on all banks.
 //
 // The tiles fill the chip in rounds of one workgroup per CU; the tiles of a last, unfilled round are cut along K into `pieces`
@@ -215,6 +224,7 @@ struct TilePlan {
 };
 
 static const int kStripRows = 4;
+static const int kLoadGroups = 8;
 
 // Workgroups are dealt to the 8 XCDs in turn: give each a contiguous range of the order, which runs down strips of kStripRows
 // row tiles, so that the 32 tiles an XCD works on share 4 rows' and 8 columns' operands in its L2.
@@ -230,7 +240,6 @@ __device__ __forceinline__ void tile_of(const TilePlan &t, int order, int &m, in
   m = strip * kStripRows + at - n * rows;
 }
 
-typedef __attribute__((address_space(1))) const void *global_ptr;
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
 // The R rows of one operand's tile, a block at a time, into LDS.
@@ -239,22 +248,29 @@ struct TileLoader {
   static constexpr int N = R * 8 / THREADS;  // 16-byte chunks per thread
   static_assert(R * 8 % THREADS == 0, "whole rounds of chunks");
   const uint8_t *base;  // the tile's first row
-  unsigned offset[N];
-  int first, rows, ld;
-  __device__ __forceinline__ TileLoader(const uint8_t *operand, long long stride, int first_row, int total_rows)
+  int offset[N];
+  int first, rows, ld, bytes;
+  __device__ __forceinline__ TileLoader(const uint8_t *operand, long long stride, int first_row, int total_rows, int K)
       : base(operand + first_row * stride), first(first_row), rows(total_rows), ld((int)stride) {
+    bytes = (min(R, rows - first) - 1) * ld + K;  // under R * 2^23
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = i * THREADS + (int)threadIdx.x, row = c >> 3;
-      offset[i] = (unsigned)(min(row, rows - 1 - first) * ld + (((c & 7) ^ (row & 7)) << 4));  // rows beyond the end: the last one
+      offset[i] = min(row, rows - 1 - first) * ld + (((c & 7) ^ (row & 7)) << 4);  // rows beyond the end: the last one
     }
   }
-  __device__ __forceinline__ void start(int block, uint8_t *lds) const {
-    const uint8_t *p = base + (long long)block * kQuantBlock;
+  // Buffer loads: the block's offset is a scalar operand, and unlike the flat forms they leave the order of the wave's other
+  // loads known to the compiler, whose waits are then for what they have to be.
+  __device__ __forceinline__ void start_one(int i, int block, uint8_t *lds) const {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know the builtins' types
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, 0x00027000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_ptr)(lds + (i * THREADS + wave * 64) * 16), 16, offset[i], block * kQuantBlock, 0, 0);
+#endif
+  }
+  __device__ __forceinline__ void start(int block, uint8_t *lds) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      __builtin_amdgcn_global_load_lds((global_ptr)(p + offset[i]), (lds_ptr)(lds + (i * THREADS + wave * 64) * 16), 16, 0, 0);
+    for (int i = 0; i < N; ++i) start_one(i, block, lds);
   }
   // the last, partial block: zeros behind the row's end
   __device__ __forceinline__ void partial(int block, int K, uint8_t *lds) const {
@@ -274,14 +290,36 @@ __device__ __forceinline__ i32x8 read_operand(const uint8_t *lds, int at, int si
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
+// out[r] = v of lane 16 r + lane % 16: each of the wave's four rows of 16 lanes spread over all of them.
+template <typename V>
+__device__ __forceinline__ void rows_of_16_to_all(V v, V *out) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto halves = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // rows 0 1 0 1, rows 2 3 2 3
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const unsigned w = halves[h];
+    const auto rows = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    const unsigned r0 = rows[0], r1 = rows[1];
+    out[2 * h] = __builtin_bit_cast(V, r0);
+    out[2 * h + 1] = __builtin_bit_cast(V, r1);
+  }
+}
+
+// Waits until at most `left` of the wave's loads are in flight and all its LDS reads are back, then for the other waves.
+template <int LEFT>
+__device__ __forceinline__ void step_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 template <int MT, int NT, int WM, int WN, int MODE>
 __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs p, TilePlan plan, f32x4 *__restrict__ partial) {
   constexpr int THREADS = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
-  constexpr int HALF = (BM + BN) * kQuantBlock + BM * 4;  // a's tile, b's tile, a's scales
-  static_assert(BM <= THREADS, "a thread per row loads a scale");
+  constexpr int ROWS = 16 * MT, SCALES = (ROWS + 63) / 64;  // a wave's rows of a; registers that hold their scales
   using S = Scale<MODE>;
   using O = Operand<MODE>;
-  extern __shared__ uint8_t smem[];
+  extern __shared__ uint8_t smem[];  // three tiles of a, two of b
   int tile, k0 = 0, k1 = p.blocks, piece = -1;
   if ((int)blockIdx.x < plan.whole) {
     tile = xcd_contiguous((int)blockIdx.x, plan.whole);
@@ -297,13 +335,19 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
   tile_of(plan, tile, tm, tn);
   const int m0 = __builtin_amdgcn_readfirstlane(tm) * BM, n0 = __builtin_amdgcn_readfirstlane(tn) * BN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
-  const int wm = (wave % WM) * MT * 16, wn = (wave / WM) * NT * 16;  // the wave's corner in the tile
-  const TileLoader<BM, THREADS> load_a(p.a, p.lda, m0, p.M);
-  const TileLoader<BN, THREADS> load_b(p.b, p.ldb, n0, p.N);
-  const int whole_blocks = p.K / kQuantBlock;
-  // NT * 16 divides 128: one row of b's scales
-  const long long sb_at = (long long)(min(n0 + wn, p.N - 1) / kQuantBlock) * p.sb_row;
-  const long long sa_at = (long long)min(m0 + (int)threadIdx.x, p.M - 1) * p.sa_row;
+  const int wm = (wave % WM) * ROWS, wn = (wave / WM) * NT * 16;  // the wave's corner in the tile
+  const TileLoader<BM, THREADS> load_a(p.a, p.lda, m0, p.M, p.K);
+  const TileLoader<BN, THREADS> load_b(p.b, p.ldb, n0, p.N, p.K);
+  const int last = min(k1, p.K / kQuantBlock);  // whole blocks end here
+
+  // NT * 16 divides 128: one row of b's scales.  The lane's part of the address is zero, but keeps it a vector load: scalar
+  // loads would make every wait for LDS one for all of them
+  int zero = 0;
+  asm("" : "+v"(zero));
+  const long long sb_at = (long long)(min(n0 + wn, p.N - 1) / kQuantBlock) * p.sb_row + zero;
+  long long sa_at[SCALES];
+#pragma unroll
+  for (int i = 0; i < SCALES; ++i) sa_at[i] = (long long)min(m0 + wm + min(i * 64 + lane, ROWS - 1), p.M - 1) * p.sa_row;
 
   f32x4 acc[MT][NT];
 #pragma unroll
@@ -311,40 +355,96 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
-  typename S::type sa_next = 0, sb_next = 0;
-  auto fetch = [&](int block, uint8_t *to) {
-    if (block < whole_blocks) {
-      load_a.start(block, to);
-      load_b.start(block, to + BM * kQuantBlock);
-    } else {
-      load_a.partial(block, p.K, to);
-      load_b.partial(block, p.K, to + BM * kQuantBlock);
-    }
-    if (BM == THREADS || threadIdx.x < BM) sa_next = S::load(p.sa, sa_at + block * p.sa_block);
+  typename S::type sa_next[SCALES], sb_next;
+  auto fetch_scales = [&](int block) {
+#pragma unroll
+    for (int i = 0; i < SCALES; ++i) sa_next[i] = S::load(p.sa, sa_at[i] + block * p.sa_block);
     sb_next = S::load(p.sb, sb_at + block * p.sb_block);
   };
+  // The lane's scale of row i * 16 + lane % 16 for every i, and b's scale
+  typename S::type sa[SCALES * 4], sb;
+  auto take_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < SCALES; ++i) rows_of_16_to_all(sa_next[i], sa + 4 * i);
+    sb = sb_next;
+  };
   const int lane_at = (lane & 15) * kQuantBlock + (((lane >> 4) ^ (lane & 7)) << 4);
-  if (k0 < k1) fetch(k0, smem);
-  for (int kb = k0; kb < k1; ++kb) {
-    uint8_t *half = smem + ((kb - k0) & 1) * HALF;
-    typename S::type *scales = reinterpret_cast<typename S::type *>(half + (BM + BN) * kQuantBlock);
-    if (BM == THREADS || threadIdx.x < BM) scales[threadIdx.x] = sa_next;
-    const typename S::type sb = sb_next;
-    // this block has arrived, and every wave is done with the other half
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (kb + 1 < k1) fetch(kb + 1, smem + ((kb + 1 - k0) & 1) * HALF);
-    const uint8_t *a = half + wm * kQuantBlock, *b = half + (BM + wn) * kQuantBlock;
+  // a's next operand is read while this one is multiplied, and a group's scaled sums follow the next group's products
+  auto compute = [&](const uint8_t *a_tile, const uint8_t *b_tile, auto &&between) {
+    const uint8_t *a = a_tile + wm * kQuantBlock, *b = b_tile + wn * kQuantBlock;
+    i32x8 x = read_operand(a, lane_at, 0);
     typename O::type w[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) w[j] = O::of(read_operand(b, lane_at, j));
+    f32x4 before[NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const typename O::type x = O::of(read_operand(a, lane_at, i));
-      const typename S::type sa = scales[wm + i * 16 + (lane & 15)];
+      i32x8 coming;
+      if (i + 1 < MT) coming = read_operand(a, lane_at, i + 1);
+      between(i);
+      const typename O::type v = O::of(x);
+      f32x4 now[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = multiply<MODE>(w[j], x, acc[i][j], sb, sa);
+      for (int j = 0; j < NT; ++j) {
+        if constexpr (MODE == kNarrowE8M0)
+          acc[i][j] = block_product<MODE>(w[j], v, acc[i][j], sb, sa[i]);
+        else
+          now[j] = block_product<MODE>(w[j], v, f32x4{0, 0, 0, 0}, sb, sa[i]);
+      }
+      if constexpr (MODE != kNarrowE8M0) {
+        if (i > 0)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) add_scaled(acc[i - 1][j], before[j], sb * sa[i - 1]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) before[j] = now[j];
+      }
+      x = coming;
+      __builtin_amdgcn_sched_barrier(0);
     }
+    if constexpr (MODE != kNarrowE8M0)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) add_scaled(acc[MT - 1][j], before[j], sb * sa[MT - 1]);
+  };
+  constexpr int A = BM * kQuantBlock, B = BN * kQuantBlock;
+  uint8_t *const bs = smem + 3 * A;
+  if (k0 < last) {
+    // Block k of a lives in tile k % 3, of b in tile k % 2.  Step k computes block k while b's block k + 1 and a's block k + 2
+    // are on their way; a's has two steps' time, so that loads are always in flight.  Past the end the last block is fetched
+    // again and not used.
+    load_a.start(k0, smem);
+    load_b.start(k0, bs);
+    fetch_scales(k0);
+    load_a.start(min(k0 + 1, last - 1), smem + A);
+    int at = 0, bt = 0;  // offsets of this step's tiles
+    for (int kb = k0; kb < last; ++kb) {
+      step_barrier<TileLoader<BM, THREADS>::N>();
+      take_scales();  // before this step's loads are issued: a wait for the scales is then none for them
+      __builtin_amdgcn_sched_barrier(0);
+      const int next = min(kb + 1, last - 1), after = min(kb + 2, last - 1);
+      fetch_scales(next);
+      uint8_t *const to_a = smem + (at == 0 ? 2 * A : at - A), *const to_b = bs + (B - bt);
+      // the loads are issued between the groups of products: all at once they would fill the memory pipe's queue and hold up
+      // the first products
+      compute(smem + at, bs + bt, [&](int i) {
+        constexpr int NA = TileLoader<BM, THREADS>::N, NB = TileLoader<BN, THREADS>::N, PER = (NA + NB + kLoadGroups - 1) / kLoadGroups;
+#pragma unroll
+        for (int l = i * PER; l < (i + 1) * PER; ++l) {
+          if (l < NB) load_b.start_one(l, next, to_b);
+          else if (l < NB + NA) load_a.start_one(l - NB, after, to_a);
+        }
+      });
+      at = at == 2 * A ? 0 : at + A;
+      bt = B - bt;
+    }
+    step_barrier<0>();
+  }
+  if (last < k1) {  // the partial block behind the whole ones
+    load_a.partial(last, p.K, smem);
+    load_b.partial(last, p.K, bs);
+    fetch_scales(last);
+    take_scales();
+    step_barrier<0>();
+    compute(smem, bs, [](int) {});
   }
   if (piece >= 0) {
     f32x4 *out = partial + (long long)piece * (MT * NT * THREADS) + threadIdx.x;
@@ -451,7 +551,7 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
 #define FRCNN_TILE(MT, NT, WM, WN)                                                                                              \
   {                                                                                                                             \
     const TilePlan plan = tile_plan(M, N, p.blocks, 16 * MT * WM, 16 * NT * WN);                                                \
-    const size_t lds = 2 * ((16 * MT * WM + 16 * NT * WN) * kQuantBlock + 64 * MT * WM);                                                   \
+    const size_t lds = (3 * 16 * MT * WM + 2 * 16 * NT * WN) * kQuantBlock;                                                     \
     const dim3 grid((unsigned)(plan.whole + plan.rest * plan.pieces));                                                          \
     if (mode == kNarrowF32) FRCNN_TILE_MODE(MT, NT, WM, WN, kNarrowF32)                                                         \
     else if (mode == kNarrowE8M0) FRCNN_TILE_MODE(MT, NT, WM, WN, kNarrowE8M0)                                                  \
