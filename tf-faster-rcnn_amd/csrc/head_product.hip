@@ -25,6 +25,7 @@ struct ProductArgs {
   long long ldy;
   int M, N, K, blocks;  // blocks = ceil(K / 128)
   int act, out;
+  int quads;  // N, ldy and the pointers allow four columns at a time
 };
 
 // The 16 bytes at `col` of a row of K bytes; bytes at K and beyond are zero.
@@ -131,7 +132,21 @@ __device__ __forceinline__ void multiply(const typename Operand<MODE>::type &w, 
 // Bias, activation, rounding and store of four neighbouring columns n .. n + 3 of row m.
 template <typename T>
 __device__ __forceinline__ void store4(const ProductArgs &p, int m, int n, f32x4 v) {
+  if (m >= p.M || n >= p.N) return;
   T *row = reinterpret_cast<T *>(p.y) + (long long)m * p.ldy + n;
+  if (p.quads) {
+    if (p.bias) v += *reinterpret_cast<const f32x4 *>(p.bias + n);
+    if (p.act == FRCNN_ACT_RELU)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = v[i] > 0.0f ? v[i] : (v[i] != v[i] ? v[i] : 0.0f);
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<f32x4 *>(row) = v;
+    } else {
+      typedef T tx4 __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<tx4 *>(row) = __builtin_convertvector(v, tx4);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (n + i < p.N) {
@@ -141,11 +156,12 @@ __device__ __forceinline__ void store4(const ProductArgs &p, int m, int n, f32x4
     }
 }
 
-__device__ __forceinline__ void finish4(const ProductArgs &p, int m, int n, f32x4 v) {
-  if (m >= p.M || n >= p.N) return;
-  if (p.out == FRCNN_F32) store4<float>(p, m, n, v);
-  else if (p.out == FRCNN_F16) store4<_Float16>(p, m, n, v);
-  else store4<__bf16>(p, m, n, v);
+// f(T) for the output's type T: one uniform branch around all of a thread's stores.
+template <typename F>
+__device__ __forceinline__ void with_output_type(const ProductArgs &p, F f) {
+  if (p.out == FRCNN_F32) f((float *)nullptr);
+  else if (p.out == FRCNN_F16) f((_Float16 *)nullptr);
+  else f((__bf16 *)nullptr);
 }
 
 // TM x TN tiles of 16 x 16 per workgroup; its W waves share the blocks of K and add their sums in LDS, in the waves' order.
@@ -203,7 +219,9 @@ __global__ __launch_bounds__(64 * W) void product_split_kernel(ProductArgs p, in
     f32x4 v = part[0][t][lane];
 #pragma unroll
     for (int w = 1; w < W; ++w) v += part[w][t][lane];
-    finish4(p, m0 + (t / TN) * 16 + (lane & 15), n0 + (t % TN) * 16 + (lane >> 4) * 4, v);
+    with_output_type(p, [&](auto *type) {
+      store4<__remove_pointer(decltype(type))>(p, m0 + (t / TN) * 16 + (lane & 15), n0 + (t % TN) * 16 + (lane >> 4) * 4, v);
+    });
   }
 }
 
@@ -224,7 +242,6 @@ struct TilePlan {
 };
 
 static const int kStripRows = 4;
-static const int kLoadGroups = 8;
 
 // Workgroups are dealt to the 8 XCDs in turn: give each a contiguous range of the order, which runs down strips of kStripRows
 // row tiles, so that the 32 tiles an XCD works on share 4 rows' and 8 columns' operands in its L2.
@@ -245,8 +262,14 @@ typedef __attribute__((address_space(3))) void *lds_ptr;
 // The R rows of one operand's tile, a block at a time, into LDS.
 template <int R, int THREADS>
 struct TileLoader {
-  static constexpr int N = R * 8 / THREADS;  // 16-byte chunks per thread
-  static_assert(R * 8 % THREADS == 0, "whole rounds of chunks");
+  static constexpr int N = (R * 8 + THREADS - 1) / THREADS;  // 16-byte chunks per thread
+  static_assert(R % 8 == 0, "whole waves of chunks");
+  // the first chunk of the thread's (wave's) i-th load; waves beyond the last chunk load others' again, so that every wave has
+  // the same number of loads in flight
+  __device__ __forceinline__ static int chunk(int i, int thread) {
+    const int c = i * THREADS + thread;
+    return (i + 1) * THREADS <= R * 8 || c < R * 8 ? c : c - (N * THREADS - R * 8);
+  }
   const uint8_t *base;  // the tile's first row
   int offset[N];
   int first, rows, ld, bytes;
@@ -255,7 +278,7 @@ struct TileLoader {
     bytes = (min(R, rows - first) - 1) * ld + K;  // under R * 2^23
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = i * THREADS + (int)threadIdx.x, row = c >> 3;
+      const int c = chunk(i, (int)threadIdx.x), row = c >> 3;
       offset[i] = min(row, rows - 1 - first) * ld + (((c & 7) ^ (row & 7)) << 4);  // rows beyond the end: the last one
     }
   }
@@ -265,7 +288,7 @@ struct TileLoader {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know the builtins' types
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, 0x00027000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_ptr)(lds + (i * THREADS + wave * 64) * 16), 16, offset[i], block * kQuantBlock, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_ptr)(lds + chunk(i, wave * 64) * 16), 16, offset[i], block * kQuantBlock, 0, 0);
 #endif
   }
   __device__ __forceinline__ void start(int block, uint8_t *lds) const {
@@ -276,7 +299,7 @@ struct TileLoader {
   __device__ __forceinline__ void partial(int block, int K, uint8_t *lds) const {
 #pragma unroll 1
     for (int i = 0; i < N; ++i) {
-      const int c = i * THREADS + (int)threadIdx.x, row = c >> 3;
+      const int c = chunk(i, (int)threadIdx.x), row = c >> 3;
       const uint8_t *r = base + (long long)min(row, rows - 1 - first) * ld;
       *reinterpret_cast<u32x4 *>(lds + c * 16) = load_chunk(r, block * kQuantBlock + ((c & 7) ^ (row & 7)) * 16, K);
     }
@@ -313,13 +336,13 @@ __device__ __forceinline__ void step_barrier() {
   asm volatile("" ::: "memory");
 }
 
-template <int MT, int NT, int WM, int WN, int MODE>
-__global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs p, TilePlan plan, f32x4 *__restrict__ partial) {
+template <int MT, int NT, int WM, int WN, int PER_CU, int DB, int MODE>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_tile_kernel(ProductArgs p, TilePlan plan, f32x4 *__restrict__ partial) {
   constexpr int THREADS = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
   constexpr int ROWS = 16 * MT, SCALES = (ROWS + 63) / 64;  // a wave's rows of a; registers that hold their scales
   using S = Scale<MODE>;
   using O = Operand<MODE>;
-  extern __shared__ uint8_t smem[];  // three tiles of a, two of b
+  extern __shared__ uint8_t smem[];  // three tiles of a, DB of b
   int tile, k0 = 0, k1 = p.blocks, piece = -1;
   if ((int)blockIdx.x < plan.whole) {
     tile = xcd_contiguous((int)blockIdx.x, plan.whole);
@@ -408,33 +431,34 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
   constexpr int A = BM * kQuantBlock, B = BN * kQuantBlock;
   uint8_t *const bs = smem + 3 * A;
   if (k0 < last) {
-    // Block k of a lives in tile k % 3, of b in tile k % 2.  Step k computes block k while b's block k + 1 and a's block k + 2
-    // are on their way; a's has two steps' time, so that loads are always in flight.  Past the end the last block is fetched
-    // again and not used.
+    // Block k of a lives in tile k % 3, of b in tile k % DB.  Step k computes block k while a's block k + 2 and b's block
+    // k + DB - 1 are on their way: what has two steps' time keeps loads in flight all along.  Past the end the last block is
+    // fetched again and not used.
+    constexpr int NA = TileLoader<BM, THREADS>::N, NB = TileLoader<BN, THREADS>::N, PER = (NA + NB + MT - 1) / MT;
     load_a.start(k0, smem);
     load_b.start(k0, bs);
     fetch_scales(k0);
+    if (DB == 3) load_b.start(min(k0 + 1, last - 1), bs + B);
     load_a.start(min(k0 + 1, last - 1), smem + A);
     int at = 0, bt = 0;  // offsets of this step's tiles
     for (int kb = k0; kb < last; ++kb) {
-      step_barrier<TileLoader<BM, THREADS>::N>();
+      step_barrier<DB == 3 ? NA + NB : NA>();
       take_scales();  // before this step's loads are issued: a wait for the scales is then none for them
       __builtin_amdgcn_sched_barrier(0);
-      const int next = min(kb + 1, last - 1), after = min(kb + 2, last - 1);
-      fetch_scales(next);
-      uint8_t *const to_a = smem + (at == 0 ? 2 * A : at - A), *const to_b = bs + (B - bt);
+      const int after = min(kb + 2, last - 1), b_next = DB == 3 ? after : min(kb + 1, last - 1);
+      fetch_scales(min(kb + 1, last - 1));
+      uint8_t *const to_a = smem + (at == 0 ? 2 * A : at - A), *const to_b = bs + (bt == 0 ? (DB - 1) * B : bt - B);
       // the loads are issued between the groups of products: all at once they would fill the memory pipe's queue and hold up
       // the first products
       compute(smem + at, bs + bt, [&](int i) {
-        constexpr int NA = TileLoader<BM, THREADS>::N, NB = TileLoader<BN, THREADS>::N, PER = (NA + NB + kLoadGroups - 1) / kLoadGroups;
 #pragma unroll
         for (int l = i * PER; l < (i + 1) * PER; ++l) {
-          if (l < NB) load_b.start_one(l, next, to_b);
+          if (l < NB) load_b.start_one(l, b_next, to_b);
           else if (l < NB + NA) load_a.start_one(l - NB, after, to_a);
         }
       });
       at = at == 2 * A ? 0 : at + A;
-      bt = B - bt;
+      bt = bt == (DB - 1) * B ? 0 : bt + B;
     }
     step_barrier<0>();
   }
@@ -453,10 +477,13 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
 #pragma unroll
       for (int j = 0; j < NT; ++j) out[(i * NT + j) * THREADS] = acc[i][j];
   } else {
+    with_output_type(p, [&](auto *type) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) finish4(p, m0 + wm + i * 16 + (lane & 15), n0 + wn + j * 16 + (lane >> 4) * 4, acc[i][j]);
+        for (int j = 0; j < NT; ++j)
+          store4<__remove_pointer(decltype(type))>(p, m0 + wm + i * 16 + (lane & 15), n0 + wn + j * 16 + (lane >> 4) * 4, acc[i][j]);
+    });
   }
 }
 
@@ -474,20 +501,107 @@ __global__ __launch_bounds__(64 * WM * WN) void product_join_kernel(ProductArgs 
   f32x4 v = in[0];
 #pragma unroll 4
   for (int i = 1; i < plan.pieces; ++i) v += in[(long long)i * (MT * NT * THREADS)];
-  finish4(p, m, n, v);
+  with_output_type(p, [&](auto *type) { store4<__remove_pointer(decltype(type))>(p, m, n, v); });
 }
 
-static TilePlan tile_plan(int M, int N, int blocks, int bm, int bn) {
+// The tile forms, and how long one takes for a block of 128 columns when the chip is full of them (measured between K = 8320 and
+// 16640, fp32 scales; `wide`: for fp32 results).  Large tiles move the fewest bytes per product: per product the 160 x 256 tile
+// takes 1.04 times as long as the 256 x 256 one, 128 x 128 1.28 and 64 x 128 1.95 times.  Small ones fill the chip when there are
+// few rows, and waste less of a ragged edge.  `best_form` takes the form with the shortest time by these figures.
+struct TileForm {
+  int bm, bn, per_cu;
+  float block_us, wide_us;
+};
+static const TileForm kTileForms[] = {{256, 256, 1, 1.63f, 0.0f}, {160, 256, 1, 1.06f, 0.0f}, {128, 128, 2, 1.04f, 1.96f}, {64, 128, 2, 0.80f, 1.17f}};
+static const int kTileFormCount = sizeof(kTileForms) / sizeof(kTileForms[0]);
+
+static TilePlan tile_plan(const TileForm &f, int M, int N, int blocks) {
   TilePlan t;
-  t.tiles_m = (M + bm - 1) / bm;
-  t.tiles_n = (N + bn - 1) / bn;
+  t.tiles_m = (M + f.bm - 1) / f.bm;
+  t.tiles_n = (N + f.bn - 1) / f.bn;
   const long long tiles = (long long)t.tiles_m * t.tiles_n;
-  t.whole = (int)(tiles / kProductCus * kProductCus);
+  const int slots = kProductCus * f.per_cu;
+  t.whole = (int)(tiles / slots * slots);
   t.rest = (int)(tiles - t.whole);
-  t.pieces = t.rest ? kProductCus / t.rest : 1;
+  t.pieces = t.rest ? slots / t.rest : 1;
   if (t.pieces > blocks / 4) t.pieces = blocks / 4;  // at least four blocks each: the first one's latency is not hidden
   if (t.pieces < 1) t.pieces = 1;
   return t;
+}
+
+static size_t plan_bytes(const TileForm &f, const TilePlan &t) {
+  return t.pieces > 1 ? (size_t)t.rest * t.pieces * f.bm * f.bn * sizeof(float) : 0;
+}
+
+static double plan_us(const TileForm &f, const TilePlan &t, int blocks, bool wide) {
+  const double block = wide ? f.wide_us : f.block_us;
+  const int slots = kProductCus * f.per_cu;
+  double us = (double)(t.whole / slots) * (blocks * block + 5.0);
+  if (t.rest) us += (blocks + t.pieces - 1) / t.pieces * block + 5.0;
+  if (t.pieces > 1) us += 4.0 + (double)t.rest * t.pieces * f.bm * f.bn * 8 / 9.5e6;  // the sums' way through memory: 9.5 TB/s
+  return us;
+}
+
+static int best_form(int M, int N, int blocks, bool wide) {
+  int best = 2;  // every result type has it
+  double least = 1e30;
+  for (int i = 0; i < kTileFormCount; ++i) {
+    if (wide && kTileForms[i].wide_us == 0.0f) continue;
+    const double us = plan_us(kTileForms[i], tile_plan(kTileForms[i], M, N, blocks), blocks, wide);
+    if (us < least) best = i, least = us;
+  }
+  return best;
+}
+
+static bool use_tiles(int M, int N) { return M >= 64 && N >= 64; }
+
+template <int MT, int NT, int WM, int WN, int PER_CU, int DB, int MODE>
+static int launch_tile(const ProductArgs &p, const TileForm &f, void *workspace, size_t workspace_bytes, hipStream_t s) {
+  if (f.bm != 16 * MT * WM || f.bn != 16 * NT * WN) return set_error(FRCNN_EINVAL, "scaled_matmul: a %d x %d tile has no kernel", f.bm, f.bn);
+  const TilePlan plan = tile_plan(f, p.M, p.N, p.blocks);
+  const size_t need = plan_bytes(f, plan);
+  if (need && !(workspace && workspace_bytes >= need))
+    return set_error(FRCNN_EINVAL, "scaled_matmul: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
+  constexpr int THREADS = 64 * WM * WN;
+  constexpr size_t lds = (3 * 16 * MT * WM + DB * 16 * NT * WN) * kQuantBlock;
+  static_assert(lds * PER_CU <= 160 * 1024, "LDS of a CU");
+  int rc = ensure_dynamic_lds((const void *)product_tile_kernel<MT, NT, WM, WN, PER_CU, DB, MODE>, lds, "scaled_matmul");
+  if (rc) return rc;
+  hipLaunchKernelGGL((product_tile_kernel<MT, NT, WM, WN, PER_CU, DB, MODE>), dim3((unsigned)(plan.whole + plan.rest * plan.pieces)),
+                     dim3(THREADS), lds, s, p, plan, (f32x4 *)workspace);
+  rc = check_launch("scaled_matmul");
+  if (rc || plan.pieces == 1) return rc;
+  hipLaunchKernelGGL((product_join_kernel<MT, NT, WM, WN>), dim3((unsigned)(plan.rest * MT * NT)), dim3(THREADS), 0, s, p, plan,
+                     (const f32x4 *)workspace);
+  return check_launch("scaled_matmul");
+}
+
+template <int MODE>
+static int launch_tiles(const ProductArgs &p, void *workspace, size_t workspace_bytes, hipStream_t s) {
+  constexpr bool wide = MODE == kWideF32 || MODE == kWideE8M0;
+  const int form = best_form(p.M, p.N, p.blocks, wide);
+  const TileForm &f = kTileForms[form];
+  if constexpr (!wide) {
+    if (form == 0) return launch_tile<8, 4, 2, 4, 1, 2, MODE>(p, f, workspace, workspace_bytes, s);
+    if (form == 1) return launch_tile<5, 4, 2, 4, 1, 3, MODE>(p, f, workspace, workspace_bytes, s);
+  }
+  if (form == 2) return launch_tile<4, 2, 2, 4, 2, 2, MODE>(p, f, workspace, workspace_bytes, s);
+  return launch_tile<2, 2, 2, 4, 2, 3, MODE>(p, f, workspace, workspace_bytes, s);
+}
+
+template <int TM, int TN, int W, int MODE>
+static int launch_split(const ProductArgs &p, hipStream_t s) {
+  const long long tm = (p.M + TM * 16 - 1) / (TM * 16), tn = (p.N + TN * 16 - 1) / (TN * 16);
+  if (tm * tn >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: too many tiles");
+  hipLaunchKernelGGL((product_split_kernel<TM, TN, W, MODE>), dim3((unsigned)(tm * tn)), dim3(64 * W), 0, s, p, (int)tn);
+  return check_launch("scaled_matmul");
+}
+
+template <int MODE>
+static int launch_product(const ProductArgs &p, void *workspace, size_t workspace_bytes, hipStream_t s) {
+  if (use_tiles(p.M, p.N)) return launch_tiles<MODE>(p, workspace, workspace_bytes, s);
+  if (p.M <= 16) return launch_split<1, 1, 16, MODE>(p, s);
+  return launch_split<4, 2, 4, MODE>(p, s);
 }
 
 }  // namespace frcnn
@@ -497,9 +611,16 @@ using namespace frcnn;
 extern "C" {
 
 size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K) {
-  if (M < 200 || N < 200 || K < 0) return 0;
-  const TilePlan t = tile_plan(M, N, (K + kQuantBlock - 1) / kQuantBlock, 256, 256);
-  return t.pieces > 1 ? (size_t)t.rest * t.pieces * 256 * 256 * sizeof(float) : 0;
+  if (K < 0 || !use_tiles(M, N)) return 0;
+  const int blocks = (K + kQuantBlock - 1) / kQuantBlock;
+  size_t most = 0;
+  for (int wide = 0; wide < 2; ++wide) {  // the output's type decides
+    const TileForm &f = kTileForms[best_form(M, N, blocks, wide != 0)];
+    const TilePlan t = tile_plan(f, M, N, blocks);
+    const size_t bytes = plan_bytes(f, t);
+    if (bytes > most) most = bytes;
+  }
+  return most;
 }
 
 int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_scale_row_stride, int64_t a_scale_block_stride,
@@ -521,56 +642,22 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
     FRCNN_REQUIRE(a_scale_row_stride >= 0 && a_scale_block_stride >= 0 && b_scale_row_stride >= 0 && b_scale_block_stride >= 0,
                   "scaled_matmul: negative scale stride");
   }
-  if (K > (1 << 22) || lda > (1 << 23) || ldb > (1 << 23) || N > (1 << 24))
+  if ((long long)((M + 63) / 64) * ((N + 63) / 64) >= (1ll << 30) || K > (1 << 22) || lda > (1 << 23) || ldb > (1 << 23) || N > (1 << 24))
     return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: K=%d (row strides %lld, %lld), N=%d is beyond what the kernels index", K,
                      (long long)lda, (long long)ldb, N);
   const size_t need = frcnn_scaled_matmul_workspace_bytes(M, N, K);
   FRCNN_REQUIRE(need == 0 || (workspace && aligned_to(workspace, 256) && workspace_bytes >= need),
                 "scaled_matmul: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);
+  const int quads = N % 4 == 0 && ldy % 4 == 0 && aligned_to(y, 4 * type_bytes(y_type)) && aligned_to(bias, 16);
   const ProductArgs p = {(const uint8_t *)a, (const uint8_t *)b, lda, ldb, a_scales, b_scales, a_scale_row_stride, a_scale_block_stride,
                          b_scale_row_stride, b_scale_block_stride, bias, y, ldy, M, N, K, (K + kQuantBlock - 1) / kQuantBlock,
-                         activation, y_type};
+                         activation, y_type, quads};
   const int mode = (y_type == FRCNN_F32 ? kWideF32 : kNarrowF32) + (scale_type == FRCNN_SCALE_E8M0);
   hipStream_t s = (hipStream_t)stream;
-#define FRCNN_SPLIT(TM, TN, W)                                                                                                 \
-  {                                                                                                                            \
-    const long long tm = (M + TM * 16 - 1) / (TM * 16), tn = (N + TN * 16 - 1) / (TN * 16);                                    \
-    if (tm * tn >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: too many tiles");                         \
-    const dim3 grid((unsigned)(tm * tn)), block(64 * W);                                                                       \
-    if (mode == kNarrowF32) hipLaunchKernelGGL((product_split_kernel<TM, TN, W, kNarrowF32>), grid, block, 0, s, p, (int)tn);  \
-    else if (mode == kNarrowE8M0) hipLaunchKernelGGL((product_split_kernel<TM, TN, W, kNarrowE8M0>), grid, block, 0, s, p, (int)tn); \
-    else if (mode == kWideF32) hipLaunchKernelGGL((product_split_kernel<TM, TN, W, kWideF32>), grid, block, 0, s, p, (int)tn); \
-    else hipLaunchKernelGGL((product_split_kernel<TM, TN, W, kWideE8M0>), grid, block, 0, s, p, (int)tn);                      \
-  }
-#define FRCNN_TILE_MODE(MT, NT, WM, WN, MODE)                                                                                   \
-  {                                                                                                                             \
-    const int rc = ensure_dynamic_lds((const void *)product_tile_kernel<MT, NT, WM, WN, MODE>, lds, "scaled_matmul");           \
-    if (rc) return rc;                                                                                                          \
-    hipLaunchKernelGGL((product_tile_kernel<MT, NT, WM, WN, MODE>), grid, dim3(64 * WM * WN), lds, s, p, plan, (f32x4 *)workspace); \
-  }
-#define FRCNN_TILE(MT, NT, WM, WN)                                                                                              \
-  {                                                                                                                             \
-    const TilePlan plan = tile_plan(M, N, p.blocks, 16 * MT * WM, 16 * NT * WN);                                                \
-    const size_t lds = (3 * 16 * MT * WM + 2 * 16 * NT * WN) * kQuantBlock;                                                     \
-    const dim3 grid((unsigned)(plan.whole + plan.rest * plan.pieces));                                                          \
-    if (mode == kNarrowF32) FRCNN_TILE_MODE(MT, NT, WM, WN, kNarrowF32)                                                         \
-    else if (mode == kNarrowE8M0) FRCNN_TILE_MODE(MT, NT, WM, WN, kNarrowE8M0)                                                  \
-    else if (mode == kWideF32) FRCNN_TILE_MODE(MT, NT, WM, WN, kWideF32)                                                        \
-    else FRCNN_TILE_MODE(MT, NT, WM, WN, kWideE8M0)                                                                             \
-    if (plan.pieces > 1) {                                                                                                      \
-      const int rc = check_launch("scaled_matmul");                                                                             \
-      if (rc) return rc;                                                                                                        \
-      hipLaunchKernelGGL((product_join_kernel<MT, NT, WM, WN>), dim3((unsigned)(plan.rest * MT * NT)), dim3(64 * WM * WN), 0, s, p, plan, \
-                         (const f32x4 *)workspace);                                                                             \
-    }                                                                                                                           \
-  }
-  if (M <= 16) FRCNN_SPLIT(1, 1, 16)
-  else if (M < 200 || N < 200) FRCNN_SPLIT(4, 2, 4)
-  else FRCNN_TILE(8, 4, 2, 4)
-#undef FRCNN_SPLIT
-#undef FRCNN_TILE
-#undef FRCNN_TILE_MODE
-  return check_launch("scaled_matmul");
+  if (mode == kNarrowF32) return launch_product<kNarrowF32>(p, workspace, workspace_bytes, s);
+  if (mode == kNarrowE8M0) return launch_product<kNarrowE8M0>(p, workspace, workspace_bytes, s);
+  if (mode == kWideF32) return launch_product<kWideF32>(p, workspace, workspace_bytes, s);
+  return launch_product<kWideE8M0>(p, workspace, workspace_bytes, s);
 }
 
 }  // extern "C"
