@@ -289,7 +289,7 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
 
 /* Group normalisation of a channels-last tensor x (N, S, C) of `type`, C in G groups of neighbouring channels: mean and
  * variance per image and group over S * (C / G) values, y = act((x - mean) / sqrt(var + epsilon) * gamma + beta).  gamma,
- * beta (C) fp32.  stats (N, G, 2) fp32 receives mean and 1 / sqrt(var + epsilon) (NULL: not wanted).  S >= 1.  Groups of up
+ * beta (C) fp32.  stats (N, G, 2) fp32, 8-byte aligned, receives mean and 1 / sqrt(var + epsilon) (NULL: not wanted).  S >= 1.  Groups of up
  * to 512 channels always, of up to 512 * 16 / sizeof(type) where 16 / sizeof(type) divides C / G and all rows are 16-byte
  * aligned. */
 size_t frcnn_group_norm_workspace_bytes(int type, int64_t N, int64_t S, int C, int G);

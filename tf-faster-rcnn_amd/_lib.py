@@ -164,7 +164,7 @@ _NO_GUARD = _NoGuard()
 def on_device(device: torch.device):
     """Context in which ``device`` is the current HIP device: the library's launches and ``hipFuncSetAttribute`` calls
     act on the current device, not on the device of the pointers they are given.  Free when it already is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == torch._C._cuda_getDevice():
         return _NO_GUARD
     return torch.cuda.device(device)
 
@@ -174,7 +174,9 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle, without a torch.cuda.Stream around it (0.1 us instead of 2)
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def ptr_table(tensors: Sequence[torch.Tensor]):

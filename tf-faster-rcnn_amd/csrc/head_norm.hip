@@ -23,19 +23,33 @@ __device__ __forceinline__ float sigmoid_fast(float z) {  // exp2 and rcp are go
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
 
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == kActRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  if (act == kActSwish) return z * sigmoid_fast(z);
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+  if (ACT == kActRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
+  if (ACT == kActSwish) return z * sigmoid_fast(z);
   return z;
 }
 
-__device__ __forceinline__ float activate_grad(float dy, float z, int act) {
-  if (act == kActRelu) return z > 0.0f ? dy : 0.0f;
-  if (act == kActSwish) {
+template <int ACT>
+__device__ __forceinline__ float activate_grad(float dy, float z) {
+  if (ACT == kActRelu) return z > 0.0f ? dy : 0.0f;
+  if (ACT == kActSwish) {
     const float s = sigmoid_fast(z);
     return dy * (s * __builtin_fmaf(z, 1.0f - s, 1.0f));
   }
   return dy;
+}
+
+// f(which) with the activation as a constant: one uniform branch around a loop instead of one per element.
+template <int A>
+struct ActivationIs {
+  static constexpr int value = A;
+};
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+  if (act == kActRelu) f(ActivationIs<kActRelu>());
+  else if (act == kActSwish) f(ActivationIs<kActSwish>());
+  else f(ActivationIs<kActNone>());
 }
 
 struct NormShape {
@@ -44,6 +58,7 @@ struct NormShape {
   int slabs;   // ceil(C / slab)
   int chunk;   // positions per workgroup
   int chunks;  // ceil(S / chunk)
+  int rows;    // positions a workgroup's threads cover at a time
 };
 
 // ---- reductions inside a workgroup ---------------------------------------------------------------------------------------
@@ -92,7 +107,14 @@ __device__ __forceinline__ void groups_of(int groups, int Cg, int threads, F val
   __syncthreads();
 }
 
-template <typename T, int VEC, int NT>
+// A pack's groups: one where the pack's width divides Cg (ONE), otherwise one per element.
+template <int VEC, bool ONE>
+struct Groups {
+  static constexpr int N = ONE ? 1 : VEC;
+  __device__ __forceinline__ static constexpr int of(int e) { return ONE ? 0 : e; }
+};
+
+template <int VEC>
 struct Column {  // a thread's place in the slab
   int row, col, rows;  // first row, first channel of its pack inside the slab, rows per pass
   int width;           // channels of this slab
@@ -100,7 +122,7 @@ struct Column {  // a thread's place in the slab
   __device__ __forceinline__ Column(const NormShape &s, int slab_index) {
     width = min(s.slab, s.C - slab_index * s.slab);
     const int vc = s.slab / VEC;  // the same for every slab, also a shorter last one
-    rows = NT / vc;
+    rows = s.rows;
     row = (int)threadIdx.x / vc;
     col = ((int)threadIdx.x - row * vc) * VEC;
     active = row < rows && col < width;
@@ -110,15 +132,15 @@ struct Column {  // a thread's place in the slab
 // ---- forward, a slab of one image (or one chunk of it) in registers --------------------------------------------------------
 // WRITE: apply and write y (the whole image is here: chunks == 1).  Otherwise only the chunk's mean and the sum of its
 // squared deviations go to `part` (N, chunks, G, 2).
-template <typename T, int VEC, int NV, int NT, bool WRITE>
-__global__ __launch_bounds__(NT) void norm_resident_kernel(const T *__restrict__ x, T *__restrict__ y, const float *__restrict__ gamma,
+template <typename T, int VEC, bool ONE, int NV, bool WRITE>
+__global__ __launch_bounds__(1024) void norm_resident_kernel(const T *__restrict__ x, T *__restrict__ y, const float *__restrict__ gamma,
                                                            const float *__restrict__ beta, float *__restrict__ stats, NormShape s,
                                                            float eps, int act) {
   extern __shared__ float lds[];
   const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
   const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
   const int chunk_index = rest % s.chunks, n = rest / s.chunks;
-  const Column<T, VEC, NT> me(s, slab_index);
+  const Column<VEC> me(s, slab_index);
   const int c0 = slab_index * s.slab + me.col;
   const int p0 = chunk_index * s.chunk;
   const int count = min(s.chunk, s.S - p0);
@@ -132,9 +154,10 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(const T *__restrict__
     const int p = me.row + i * me.rows;
     v[i] = (me.active && p < count) ? Pack<T, VEC>::load(x + base + (long long)p * s.C) : Pack<T, VEC>::zero();
   }
-  int group[VEC];
+  using Gs = Groups<VEC, ONE>;
+  int group[Gs::N];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) group[e] = me.active ? (me.col + e) / s.Cg : 0;
+  for (int e = 0; e < Gs::N; ++e) group[e] = me.active ? (me.col + e) / s.Cg : 0;
 
   float sum[1][VEC];
 #pragma unroll
@@ -148,11 +171,11 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(const T *__restrict__
   }
   rows_to_first<VEC, 1>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
   const float inv = 1.0f / ((float)count * (float)s.Cg);
-  groups_of(groups, s.Cg, NT, [&](int c) { return red[c]; }, gsum);
+  groups_of(groups, s.Cg, (int)blockDim.x, [&](int c) { return red[c]; }, gsum);
 
-  float mean[VEC];
+  float mean[Gs::N];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) mean[e] = gsum[group[e]] * inv;
+  for (int e = 0; e < Gs::N; ++e) mean[e] = gsum[group[e]] * inv;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) sum[0][e] = 0.0f;
 #pragma unroll
@@ -162,36 +185,40 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(const T *__restrict__
       v[i].unpack(f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = f[e] - mean[e];
+        const float d = f[e] - mean[Gs::of(e)];
         sum[0][e] = __builtin_fmaf(d, d, sum[0][e]);
       }
     }
   }
   rows_to_first<VEC, 1>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
-  groups_of(groups, s.Cg, NT, [&](int c) { return red[c]; }, grstd);
+  groups_of(groups, s.Cg, (int)blockDim.x, [&](int c) { return red[c]; }, grstd);
 
   const int g0 = slab_index * s.slab / s.Cg;
   if constexpr (!WRITE) {
     float *part = stats + (((long long)n * s.chunks + chunk_index) * s.G + g0) * 2;
-    for (int g = threadIdx.x; g < groups; g += NT) {
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
       part[2 * g] = gsum[g] * inv;
       part[2 * g + 1] = grstd[g];
     }
   } else {
     if (stats) {
       float *out = stats + ((long long)n * s.G + g0) * 2;
-      for (int g = threadIdx.x; g < groups; g += NT) {
+      for (int g = threadIdx.x; g < groups; g += blockDim.x) {
         out[2 * g] = gsum[g] * inv;
         out[2 * g + 1] = 1.0f / __builtin_sqrtf(__builtin_fmaf(grstd[g], inv, eps));
       }
     }
     if (!me.active) return;
-    float a[VEC], b[VEC];
+    float a[VEC], b[VEC], rstd[Gs::N];
+#pragma unroll
+    for (int e = 0; e < Gs::N; ++e) rstd[e] = 1.0f / __builtin_sqrtf(__builtin_fmaf(grstd[group[e]], inv, eps));
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      a[e] = gamma[c0 + e] / __builtin_sqrtf(__builtin_fmaf(grstd[group[e]], inv, eps));
+      a[e] = gamma[c0 + e] * rstd[Gs::of(e)];
       b[e] = beta[c0 + e];
     }
+    with_activation(act, [&](auto which) {
+      constexpr int ACT = decltype(which)::value;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int p = me.row + i * me.rows;
@@ -199,10 +226,11 @@ __global__ __launch_bounds__(NT) void norm_resident_kernel(const T *__restrict__
         float f[VEC];
         v[i].unpack(f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = activate(__builtin_fmaf(f[e] - mean[e], a[e], b[e]), act);
+        for (int e = 0; e < VEC; ++e) f[e] = activate<ACT>(__builtin_fmaf(f[e] - mean[Gs::of(e)], a[e], b[e]));
         Pack<T, VEC>::store(y + base + (long long)p * s.C, f);
       }
     }
+    });
   }
 }
 
@@ -240,78 +268,97 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const float *__restrict_
 }
 
 // y from x and the joined statistics; the thread layout of norm_resident_kernel.
-template <typename T, int VEC, int NT>
-__global__ __launch_bounds__(NT) void norm_apply_kernel(const T *__restrict__ x, T *__restrict__ y, const float *__restrict__ gamma,
-                                                        const float *__restrict__ beta, const float *__restrict__ stats, NormShape s,
-                                                        int act) {
+template <typename T, int VEC, bool ONE>
+__global__ __launch_bounds__(1024) void norm_apply_kernel(const T *__restrict__ x, T *__restrict__ y, const float *__restrict__ gamma,
+                                                          const float *__restrict__ beta, const float *__restrict__ stats, NormShape s,
+                                                          int act) {
+  using Gs = Groups<VEC, ONE>;
   const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
   const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
   const int chunk_index = rest % s.chunks, n = rest / s.chunks;
-  const Column<T, VEC, NT> me(s, slab_index);
+  const Column<VEC> me(s, slab_index);
   if (!me.active) return;
   const int c0 = slab_index * s.slab + me.col;
   const int p0 = chunk_index * s.chunk;
   const int count = min(s.chunk, s.S - p0);
   const long long base = ((long long)n * s.S + p0) * s.C + c0;
-  float mean[VEC], a[VEC], b[VEC];
+  float mean[Gs::N], rstd[Gs::N], a[VEC], b[VEC];
+#pragma unroll
+  for (int e = 0; e < Gs::N; ++e) {
+    const f32x2 st = *reinterpret_cast<const f32x2 *>(stats + ((long long)n * s.G + (c0 + e) / s.Cg) * 2);
+    mean[e] = st.x;
+    rstd[e] = st.y;
+  }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
-    const float *st = stats + ((long long)n * s.G + (c0 + e) / s.Cg) * 2;
-    mean[e] = st[0];
-    a[e] = gamma[c0 + e] * st[1];
+    a[e] = gamma[c0 + e] * rstd[Gs::of(e)];
     b[e] = beta[c0 + e];
   }
+  with_activation(act, [&](auto which) {
+    constexpr int ACT = decltype(which)::value;
 #pragma unroll 4
-  for (int p = me.row; p < count; p += me.rows) {
-    float f[VEC];
-    Pack<T, VEC>::load(x + base + (long long)p * s.C).unpack(f);
+    for (int p = me.row; p < count; p += me.rows) {
+      float f[VEC];
+      Pack<T, VEC>::load(x + base + (long long)p * s.C).unpack(f);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = activate(__builtin_fmaf(f[e] - mean[e], a[e], b[e]), act);
-    Pack<T, VEC>::store(y + base + (long long)p * s.C, f);
-  }
+      for (int e = 0; e < VEC; ++e) f[e] = activate<ACT>(__builtin_fmaf(f[e] - mean[Gs::of(e)], a[e], b[e]));
+      Pack<T, VEC>::store(y + base + (long long)p * s.C, f);
+    }
+  });
 }
 
 // ---- gradients -------------------------------------------------------------------------------------------------------------
-template <int VEC>
+template <int VEC, bool ONE>
 struct GradCoefficients {
-  float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC];
-  __device__ __forceinline__ void load(const float *__restrict__ stats, const float *__restrict__ g, const float *__restrict__ b,
-                                       const NormShape &s, int n, int c0) {
+  using Gs = Groups<VEC, ONE>;
+  float mean[Gs::N], rstd[Gs::N], gamma[VEC], beta[VEC];
+  __device__ __forceinline__ void parameters(const float *__restrict__ g, const float *__restrict__ b, int c0) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float *st = stats + ((long long)n * s.G + (c0 + e) / s.Cg) * 2;
-      mean[e] = st[0];
-      rstd[e] = st[1];
       gamma[e] = g[c0 + e];
       beta[e] = b[c0 + e];
     }
   }
-  // xhat and dz of one element
-  __device__ __forceinline__ void of(int e, float x, float dy, int act, float &xhat, float &dz) const {
-    xhat = (x - mean[e]) * rstd[e];
-    dz = activate_grad(dy, __builtin_fmaf(xhat, gamma[e], beta[e]), act);
+  __device__ __forceinline__ void statistics(const float *__restrict__ stats, const NormShape &s, int n, int c0) {
+#pragma unroll
+    for (int e = 0; e < Gs::N; ++e) {
+      const f32x2 st = *reinterpret_cast<const f32x2 *>(stats + ((long long)n * s.G + (c0 + e) / s.Cg) * 2);
+      mean[e] = st.x;
+      rstd[e] = st.y;
+    }
+  }
+  __device__ __forceinline__ float xhat(int e, float x) const { return (x - mean[Gs::of(e)]) * rstd[Gs::of(e)]; }
+  template <int ACT>
+  __device__ __forceinline__ float dz(int e, float xh, float dy) const {
+    return activate_grad<ACT>(dy, __builtin_fmaf(xh, gamma[e], beta[e]));
+  }
+  __device__ __forceinline__ float dx(int e, float xh, float dz, float d1, float d2) const {
+    return rstd[Gs::of(e)] * __builtin_fmaf(-xh, d2, __builtin_fmaf(dz, gamma[e], -d1));
   }
 };
 
-// A slab of one image's x and dy in registers; each workgroup takes `per` images in turn and leaves its sums for dgamma and
-// dbeta in sums (workgroups along N, C, 2).
-template <typename T, int VEC, int NV, int NT>
-__global__ __launch_bounds__(NT) void norm_grad_resident_kernel(const T *__restrict__ dy, const T *__restrict__ x,
-                                                                const float *__restrict__ gamma, const float *__restrict__ beta,
-                                                                const float *__restrict__ stats, T *__restrict__ dx,
-                                                                float *__restrict__ sums, NormShape s, int per, int act) {
+// A slab of one image's x and dz in registers, x as it is stored and dz in fp32, so that the activation's gradient is computed
+// once; each workgroup takes `per` images in turn and leaves its sums for dgamma and dbeta in sums (workgroups along N, C, 2).
+template <typename T, int VEC, bool ONE, int NV>
+__global__ __launch_bounds__(512) void norm_grad_resident_kernel(const T *__restrict__ dy, const T *__restrict__ x,
+                                                                 const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                                 const float *__restrict__ stats, T *__restrict__ dx,
+                                                                 float *__restrict__ sums, NormShape s, int per, int act) {
   extern __shared__ float lds[];
+  using Gs = Groups<VEC, ONE>;
   const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
   const int part = (int)(blockIdx.x / (unsigned)s.slabs);
-  const Column<T, VEC, NT> me(s, slab_index);
+  const Column<VEC> me(s, slab_index);
   const int c0 = slab_index * s.slab + me.col;
   const int groups = me.width / s.Cg;
   float *red = lds, *first = lds + 2 * me.rows * s.slab, *second = first + s.slab / s.Cg, *weight = second + s.slab / s.Cg;
   const int plane = me.rows * s.slab;
-  for (int c = threadIdx.x; c < me.width; c += NT) weight[c] = gamma[slab_index * s.slab + c];
-  int group[VEC];
+  for (int c = threadIdx.x; c < me.width; c += blockDim.x) weight[c] = gamma[slab_index * s.slab + c];
+  int group[Gs::N];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) group[e] = me.active ? (me.col + e) / s.Cg : 0;
+  for (int e = 0; e < Gs::N; ++e) group[e] = me.active ? (me.col + e) / s.Cg : 0;
+  GradCoefficients<VEC, ONE> k;
+  if (me.active) k.parameters(gamma, beta, c0);
   float total[2][VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) total[0][e] = total[1][e] = 0.0f;
@@ -328,26 +375,28 @@ __global__ __launch_bounds__(NT) void norm_grad_resident_kernel(const T *__restr
       vx[i] = in ? Pack<T, VEC>::load(x + base + (long long)p * s.C) : Pack<T, VEC>::zero();
       vd[i] = in ? Pack<T, VEC>::load(dy + base + (long long)p * s.C) : Pack<T, VEC>::zero();
     }
-    GradCoefficients<VEC> k;
-    if (me.active) k.load(stats, gamma, beta, s, n, c0);
-    float sum[2][VEC];
+    if (me.active) k.statistics(stats, s, n, c0);
+    float sum[2][VEC], dz[NV][VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[0][e] = sum[1][e] = 0.0f;
+    with_activation(act, [&](auto which) {
+      constexpr int ACT = decltype(which)::value;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (me.row + i * me.rows < s.S) {
-        float fx[VEC], fd[VEC];
-        vx[i].unpack(fx);
-        vd[i].unpack(fd);
+      for (int i = 0; i < NV; ++i) {
+        vd[i].unpack(dz[i]);
+        if (me.row + i * me.rows < s.S) {
+          float fx[VEC];
+          vx[i].unpack(fx);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          float xhat, dz;
-          k.of(e, fx[e], fd[e], act, xhat, dz);
-          sum[0][e] += dz;
-          sum[1][e] = __builtin_fmaf(dz, xhat, sum[1][e]);
+          for (int e = 0; e < VEC; ++e) {
+            const float xh = k.xhat(e, fx[e]);
+            dz[i][e] = k.template dz<ACT>(e, xh, dz[i][e]);
+            sum[0][e] += dz[i][e];
+            sum[1][e] = __builtin_fmaf(dz[i][e], xh, sum[1][e]);
+          }
         }
       }
-    }
+    });
     rows_to_first<VEC, 2>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
     if (me.active && me.row == 0)
 #pragma unroll
@@ -355,12 +404,12 @@ __global__ __launch_bounds__(NT) void norm_grad_resident_kernel(const T *__restr
         total[0][e] += sum[0][e];
         total[1][e] += sum[1][e];
       }
-    groups_of(groups, s.Cg, NT, [&](int c) { return red[c] * weight[c]; }, first);
-    groups_of(groups, s.Cg, NT, [&](int c) { return red[plane + c] * weight[c]; }, second);
+    groups_of(groups, s.Cg, (int)blockDim.x, [&](int c) { return red[c] * weight[c]; }, first);
+    groups_of(groups, s.Cg, (int)blockDim.x, [&](int c) { return red[plane + c] * weight[c]; }, second);
     if (me.active) {
-      float d1[VEC], d2[VEC];
+      float d1[Gs::N], d2[Gs::N];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
+      for (int e = 0; e < Gs::N; ++e) {
         d1[e] = first[group[e]] * inv;
         d2[e] = second[group[e]] * inv;
       }
@@ -368,16 +417,11 @@ __global__ __launch_bounds__(NT) void norm_grad_resident_kernel(const T *__restr
       for (int i = 0; i < NV; ++i) {
         const int p = me.row + i * me.rows;
         if (p < s.S) {
-          float fx[VEC], fd[VEC];
-          vx[i].unpack(fx);
-          vd[i].unpack(fd);
+          float f[VEC];
+          vx[i].unpack(f);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            float xhat, dz;
-            k.of(e, fx[e], fd[e], act, xhat, dz);
-            fd[e] = k.rstd[e] * (__builtin_fmaf(dz, k.gamma[e], -d1[e]) - xhat * d2[e]);
-          }
-          Pack<T, VEC>::store(dx + base + (long long)p * s.C, fd);
+          for (int e = 0; e < VEC; ++e) f[e] = k.dx(e, k.xhat(e, f[e]), dz[i][e], d1[Gs::of(e)], d2[Gs::of(e)]);
+          Pack<T, VEC>::store(dx + base + (long long)p * s.C, f);
         }
       }
     }
@@ -393,16 +437,16 @@ __global__ __launch_bounds__(NT) void norm_grad_resident_kernel(const T *__restr
 }
 
 // Per-channel sums of one chunk of positions, into sums (N, chunks, C, 2).
-template <typename T, int VEC, int NT>
-__global__ __launch_bounds__(NT) void norm_grad_sums_kernel(const T *__restrict__ dy, const T *__restrict__ x,
-                                                            const float *__restrict__ gamma, const float *__restrict__ beta,
-                                                            const float *__restrict__ stats, float *__restrict__ sums, NormShape s,
-                                                            int act) {
+template <typename T, int VEC, bool ONE>
+__global__ __launch_bounds__(512) void norm_grad_sums_kernel(const T *__restrict__ dy, const T *__restrict__ x,
+                                                             const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                             const float *__restrict__ stats, float *__restrict__ sums, NormShape s,
+                                                             int act) {
   extern __shared__ float lds[];
   const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
   const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
   const int chunk_index = rest % s.chunks, n = rest / s.chunks;
-  const Column<T, VEC, NT> me(s, slab_index);
+  const Column<VEC> me(s, slab_index);
   const int c0 = slab_index * s.slab + me.col;
   const int p0 = chunk_index * s.chunk;
   const int count = min(s.chunk, s.S - p0);
@@ -411,8 +455,101 @@ __global__ __launch_bounds__(NT) void norm_grad_sums_kernel(const T *__restrict_
 #pragma unroll
   for (int e = 0; e < VEC; ++e) sum[0][e] = sum[1][e] = 0.0f;
   if (me.active) {
-    GradCoefficients<VEC> k;
-    k.load(stats, gamma, beta, s, n, c0);
+    GradCoefficients<VEC, ONE> k;
+    k.parameters(gamma, beta, c0);
+    k.statistics(stats, s, n, c0);
+    with_activation(act, [&](auto which) {
+      constexpr int ACT = decltype(which)::value;
+#pragma unroll 4
+      for (int p = me.row; p < count; p += me.rows) {
+        float fx[VEC], fd[VEC];
+        Pack<T, VEC>::load(x + base + (long long)p * s.C).unpack(fx);
+        Pack<T, VEC>::load(dy + base + (long long)p * s.C).unpack(fd);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float xh = k.xhat(e, fx[e]), dz = k.template dz<ACT>(e, xh, fd[e]);
+          sum[0][e] += dz;
+          sum[1][e] = __builtin_fmaf(dz, xh, sum[1][e]);
+        }
+      }
+    });
+  }
+  rows_to_first<VEC, 2>(lds, me.rows, s.slab, me.row, me.col, me.active, sum);
+  if (me.active && me.row == 0)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      *reinterpret_cast<f32x2 *>(sums + (((long long)n * s.chunks + chunk_index) * s.C + c0 + e) * 2) = f32x2{sum[0][e], sum[1][e]};
+}
+
+// One workgroup per (image, group): the chunks' sums become E d and E (d xhat), and the image's per-channel sums.  Its threads
+// form `lanes` columns of channels times 256 / lanes rows of chunks.
+__global__ __launch_bounds__(256) void norm_grad_join_kernel(const float *__restrict__ sums, const float *__restrict__ gamma,
+                                                             float *__restrict__ image_sums, float *__restrict__ expect, NormShape s) {
+  const int g = (int)(blockIdx.x % (unsigned)s.G), n = (int)(blockIdx.x / (unsigned)s.G);
+  __shared__ f32x2 red[256];
+  int lanes = 1;
+  while (lanes < s.Cg && lanes < 256) lanes <<= 1;
+  const int lane = (int)threadIdx.x & (lanes - 1), row = (int)threadIdx.x / lanes, rows = 256 / lanes;
+  f32x2 d = {0.0f, 0.0f};
+  for (int c0 = 0; c0 < s.Cg; c0 += lanes) {
+    const int c = c0 + lane, ch = g * s.Cg + c;
+    f32x2 v = {0.0f, 0.0f};
+    if (c < s.Cg) {
+#pragma unroll 8
+      for (int k = row; k < s.chunks; k += rows) v += *reinterpret_cast<const f32x2 *>(sums + (((long long)n * s.chunks + k) * s.C + ch) * 2);
+    }
+    red[threadIdx.x] = v;
+    __syncthreads();
+    for (int half = rows >> 1; half > 0; half >>= 1) {
+      if (row < half) red[threadIdx.x] += red[threadIdx.x + half * lanes];
+      __syncthreads();
+    }
+    if (row == 0 && c < s.Cg) {
+      v = red[lane];
+      *reinterpret_cast<f32x2 *>(image_sums + ((long long)n * s.C + ch) * 2) = v;
+      d += v * gamma[ch];
+    }
+    __syncthreads();
+  }
+  red[threadIdx.x] = d;  // zeros but for the first row
+  __syncthreads();
+  for (int half = 128; half > 0; half >>= 1) {
+    if ((int)threadIdx.x < half) red[threadIdx.x] += red[threadIdx.x + half];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const float m = (float)s.S * (float)s.Cg;
+    *reinterpret_cast<f32x2 *>(expect + ((long long)n * s.G + g) * 2) = f32x2{red[0].x / m, red[0].y / m};
+  }
+}
+
+template <typename T, int VEC, bool ONE>
+__global__ __launch_bounds__(512) void norm_grad_apply_kernel(const T *__restrict__ dy, const T *__restrict__ x,
+                                                              const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                              const float *__restrict__ stats, const float *__restrict__ expect,
+                                                              T *__restrict__ dx, NormShape s, int act) {
+  using Gs = Groups<VEC, ONE>;
+  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
+  const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
+  const int chunk_index = rest % s.chunks, n = rest / s.chunks;
+  const Column<VEC> me(s, slab_index);
+  if (!me.active) return;
+  const int c0 = slab_index * s.slab + me.col;
+  const int p0 = chunk_index * s.chunk;
+  const int count = min(s.chunk, s.S - p0);
+  const long long base = ((long long)n * s.S + p0) * s.C + c0;
+  GradCoefficients<VEC, ONE> k;
+  k.parameters(gamma, beta, c0);
+  k.statistics(stats, s, n, c0);
+  float d1[Gs::N], d2[Gs::N];
+#pragma unroll
+  for (int e = 0; e < Gs::N; ++e) {
+    const f32x2 o = *reinterpret_cast<const f32x2 *>(expect + ((long long)n * s.G + (c0 + e) / s.Cg) * 2);
+    d1[e] = o.x;
+    d2[e] = o.y;
+  }
+  with_activation(act, [&](auto which) {
+    constexpr int ACT = decltype(which)::value;
 #pragma unroll 4
     for (int p = me.row; p < count; p += me.rows) {
       float fx[VEC], fd[VEC];
@@ -420,94 +557,12 @@ __global__ __launch_bounds__(NT) void norm_grad_sums_kernel(const T *__restrict_
       Pack<T, VEC>::load(dy + base + (long long)p * s.C).unpack(fd);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float xhat, dz;
-        k.of(e, fx[e], fd[e], act, xhat, dz);
-        sum[0][e] += dz;
-        sum[1][e] = __builtin_fmaf(dz, xhat, sum[1][e]);
+        const float xh = k.xhat(e, fx[e]);
+        fd[e] = k.dx(e, xh, k.template dz<ACT>(e, xh, fd[e]), d1[Gs::of(e)], d2[Gs::of(e)]);
       }
+      Pack<T, VEC>::store(dx + base + (long long)p * s.C, fd);
     }
-  }
-  rows_to_first<VEC, 2>(lds, me.rows, s.slab, me.row, me.col, me.active, sum);
-  if (me.active && me.row == 0)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float *o = sums + (((long long)n * s.chunks + chunk_index) * s.C + c0 + e) * 2;
-      o[0] = sum[0][e];
-      o[1] = sum[1][e];
-    }
-}
-
-// One workgroup per (image, group): the chunks' sums become E d and E (d xhat), and the image's per-channel sums.
-__global__ __launch_bounds__(256) void norm_grad_join_kernel(const float *__restrict__ sums, const float *__restrict__ gamma,
-                                                             float *__restrict__ image_sums, float *__restrict__ expect, NormShape s) {
-  const int g = (int)(blockIdx.x % (unsigned)s.G), n = (int)(blockIdx.x / (unsigned)s.G);
-  __shared__ float red[2][4];
-  float d1 = 0.0f, d2 = 0.0f;
-  for (int c = threadIdx.x; c < s.Cg; c += 256) {
-    const int ch = g * s.Cg + c;
-    float a = 0.0f, b = 0.0f;
-#pragma unroll 8
-    for (int k = 0; k < s.chunks; ++k) {
-      const f32x2 v = *reinterpret_cast<const f32x2 *>(sums + (((long long)n * s.chunks + k) * s.C + ch) * 2);
-      a += v.x;
-      b += v.y;
-    }
-    *reinterpret_cast<f32x2 *>(image_sums + ((long long)n * s.C + ch) * 2) = f32x2{a, b};
-    d1 = __builtin_fmaf(a, gamma[ch], d1);
-    d2 = __builtin_fmaf(b, gamma[ch], d2);
-  }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    d1 += __shfl_xor(d1, d);
-    d2 += __shfl_xor(d2, d);
-  }
-  if ((threadIdx.x & 63) == 0) {
-    red[0][threadIdx.x >> 6] = d1;
-    red[1][threadIdx.x >> 6] = d2;
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    const float *r = red[threadIdx.x];
-    expect[((long long)n * s.G + g) * 2 + threadIdx.x] = (r[0] + r[1] + (r[2] + r[3])) / ((float)s.S * (float)s.Cg);
-  }
-}
-
-template <typename T, int VEC, int NT>
-__global__ __launch_bounds__(NT) void norm_grad_apply_kernel(const T *__restrict__ dy, const T *__restrict__ x,
-                                                             const float *__restrict__ gamma, const float *__restrict__ beta,
-                                                             const float *__restrict__ stats, const float *__restrict__ expect,
-                                                             T *__restrict__ dx, NormShape s, int act) {
-  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
-  const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
-  const int chunk_index = rest % s.chunks, n = rest / s.chunks;
-  const Column<T, VEC, NT> me(s, slab_index);
-  if (!me.active) return;
-  const int c0 = slab_index * s.slab + me.col;
-  const int p0 = chunk_index * s.chunk;
-  const int count = min(s.chunk, s.S - p0);
-  const long long base = ((long long)n * s.S + p0) * s.C + c0;
-  GradCoefficients<VEC> k;
-  k.load(stats, gamma, beta, s, n, c0);
-  float d1[VEC], d2[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const float *o = expect + ((long long)n * s.G + (c0 + e) / s.Cg) * 2;
-    d1[e] = o[0];
-    d2[e] = o[1];
-  }
-#pragma unroll 4
-  for (int p = me.row; p < count; p += me.rows) {
-    float fx[VEC], fd[VEC];
-    Pack<T, VEC>::load(x + base + (long long)p * s.C).unpack(fx);
-    Pack<T, VEC>::load(dy + base + (long long)p * s.C).unpack(fd);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float xhat, dz;
-      k.of(e, fx[e], fd[e], act, xhat, dz);
-      fd[e] = k.rstd[e] * (__builtin_fmaf(dz, k.gamma[e], -d1[e]) - xhat * d2[e]);
-    }
-    Pack<T, VEC>::store(dx + base + (long long)p * s.C, fd);
-  }
+  });
 }
 
 // dbeta[c], dgamma[c] = the sums of `parts` rows of (C, 2): 8 channels per workgroup, 64 threads down the rows of each.
@@ -531,109 +586,153 @@ __global__ __launch_bounds__(1024) void norm_grad_params_kernel(const float *__r
 }
 
 // ---- the choice of a split -------------------------------------------------------------------------------------------------
-static const int kNormThreads = 512;
-static const int kNormMaxColumns = kNormThreads;  // packs of a slab: at least one row of threads
-static const int kNormTargetGroups = 1024;        // workgroups that fill the chip twice over at two per CU
+static const int kNormColumns = 512;   // packs of a slab at most: one row of threads
+static const int kNormLine = 128;      // bytes of a slab's row that are worth a read of their own
 
 struct NormPlan {
   NormShape s;
-  int vec;    // elements per pack; 0: not supported
-  int nv;     // packs a thread holds: 1, 2, 4, 8 (forward: 16)
+  int vec;      // elements per pack; 0: not supported
+  bool one;     // a pack lies in one group
+  int threads;
+  int nv;       // packs a thread holds
   bool resident;
-  int rows;   // rows of threads
 };
 
 static int gcd_int(int a, int b) { return b ? gcd_int(b, a % b) : a; }
 
-// Whole image per workgroup where a slab's packs fit `most` per thread, chunks of positions otherwise.
-static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, int most) {
+// Threads for a slab of `columns` packs of S positions, `most` packs per thread: the least idle lanes, about six packs each (bytes
+// in flight against waves).  0: none fits.
+static int norm_threads(int columns, int S, int most, int limit) {
+  int best = 0;
+  float least = 0;
+  for (int t = 64; t <= limit; t += 64) {
+    const int rows = t / columns;
+    if (!rows) continue;
+    const int need = (S + rows - 1) / rows;
+    if (need > most) continue;
+    const float cost = (float)t * need / ((float)columns * S) + 0.02f * (need > 6 ? need - 6 : 6 - need);
+    if (!best || cost < least) best = t, least = cost;
+  }
+  return best;
+}
+
+// Whole images per workgroup where a slab's packs fit its registers, chunks of positions otherwise.  grad: two tensors are held,
+// in up to 512 threads of 8 packs; the forward pass holds one, in up to 512 threads of 8 or 1024 of 16.
+static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, bool grad) {
   NormPlan p = {};
   p.s.N = N, p.s.S = S, p.s.C = C, p.s.G = G, p.s.Cg = C / G;
   int vec = aligned && ((long long)C * elem) % 16 == 0 ? 16 / elem : 1;
   long long unit = (long long)p.s.Cg / gcd_int(p.s.Cg, vec) * vec;  // channels: whole groups and whole packs
-  if (unit / vec > kNormMaxColumns && vec > 1) {
+  if (unit / vec > kNormColumns && vec > 1) {
     vec = 1;
     unit = p.s.Cg;
   }
-  if (unit / vec > kNormMaxColumns) return p;
+  if (unit / vec > kNormColumns) return p;
   p.vec = vec;
+  p.one = p.s.Cg % vec == 0;
   const long long units = C / unit;
-  long long k = kNormMaxColumns * (long long)vec / unit;  // units per slab
-  if (k > units) k = units;
-  auto fits = [&](long long kk) { return (S + kNormThreads / (int)(kk * unit / vec) - 1) / (kNormThreads / (int)(kk * unit / vec)) <= most; };
-  auto groups = [&](long long kk) { return (long long)N * ((units + kk - 1) / kk); };
-  while (k > 1 && !fits(k)) k = (k + 1) / 2;
-  p.resident = fits(k);
+  long long widest = kNormColumns * (long long)vec / unit;  // units per slab
+  if (widest > units) widest = units;
+  auto threads = [&](long long k) {
+    const int t = norm_threads((int)(k * unit / vec), S, 8, 512);
+    return t || grad ? t : norm_threads((int)(k * unit / vec), S, 16, 1024);
+  };
+  // the widest slab that fits; narrower ones while the chip is not full and a row is still a line
+  long long k = widest;
+  while (k > 1 && !threads(k)) k = (k + 1) / 2;
+  p.resident = threads(k) && (k == units || k * unit * elem >= kNormLine);
   if (p.resident) {
-    // narrower slabs while the chip is not full and a slab's row is still a full 128-byte line
-    while (k > 1 && groups(k) < kNormTargetGroups && (k + 1) / 2 * unit * elem >= 128) k = (k + 1) / 2;
+    while (k > 1 && (long long)N * ((units + k - 1) / k) < 1024 && (k + 1) / 2 * unit * elem >= kNormLine && threads((k + 1) / 2)) k = (k + 1) / 2;
+    p.threads = threads(k);
     p.s.chunk = S;
-    p.s.chunks = 1;
   } else {
-    k = kNormMaxColumns * (long long)vec / unit;
-    if (k > units) k = units;
+    k = widest;
+    p.threads = 512;
   }
   p.s.slab = (int)(k * unit);
   p.s.slabs = (int)((units + k - 1) / k);
-  p.rows = kNormThreads / (p.s.slab / vec);
+  p.s.rows = p.threads / (p.s.slab / vec);
   if (!p.resident) {
-    int per = most;  // passes per chunk: as many as fit, fewer while the chip is not full
-    while (per > 2 && (long long)N * p.s.slabs * ((S + p.rows * per - 1) / (p.rows * per)) < kNormTargetGroups) per /= 2;
-    p.s.chunk = p.rows * per;
-    p.s.chunks = (S + p.s.chunk - 1) / p.s.chunk;
+    int per = 8;  // packs per thread and chunk; fewer while the chip is not full, at least four for a chunk's fixed costs
+    while (per > 4 && (long long)N * p.s.slabs * ((S + p.s.rows * per - 1) / (p.s.rows * per)) < 512) per /= 2;
+    p.s.chunk = p.s.rows * per;
   }
-  const int need = (p.s.chunk + p.rows - 1) / p.rows;
-  p.nv = 1;
-  while (p.nv < need) p.nv *= 2;
+  p.s.chunks = (S + p.s.chunk - 1) / p.s.chunk;
+  p.nv = (p.s.chunk + p.s.rows - 1) / p.s.rows;
+  if (p.nv > 8) p.nv = p.nv > 12 ? 16 : 12;
+  if (vec == 1) p.nv = p.nv > 8 ? 16 : p.nv > 4 ? 8 : p.nv > 1 ? 4 : 1;
   return p;
 }
 
-static const int kNormForwardMost = 16, kNormGradMost = 8;
+// images per workgroup: about a thousand rows of partial sums are left for the last kernel
+static int grad_images_per_group(const NormPlan &p) { return (int)(((long long)p.s.N * p.s.slabs + 1023) / 1024); }
 
-static int grad_images_per_group(const NormPlan &p) {
-  const long long per = ((long long)p.s.N * p.s.slabs + 4095) / 4096;
-  return (int)per;
+template <typename T, int VEC, bool ONE, int NV, bool WRITE>
+static int launch_resident(const NormPlan &p, const void *x, void *y, const float *gamma, const float *beta, float *out, float eps, int act,
+                           hipStream_t stream) {
+  const size_t lds = ((size_t)p.s.rows * p.s.slab + 2 * (p.s.slab / p.s.Cg)) * sizeof(float);
+  const dim3 grid((unsigned)((long long)p.s.N * p.s.chunks * p.s.slabs));
+  const int rc = ensure_dynamic_lds((const void *)norm_resident_kernel<T, VEC, ONE, NV, WRITE>, lds, "group_norm");
+  if (rc) return rc;
+  hipLaunchKernelGGL((norm_resident_kernel<T, VEC, ONE, NV, WRITE>), grid, dim3(p.threads), lds, stream, (const T *)x, (T *)y, gamma, beta,
+                     out, p.s, eps, act);
+  return check_launch("group_norm");
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool ONE>
 static int launch_norm(const NormPlan &p, const void *x, void *y, const float *gamma, const float *beta, float *stats,
                        float *workspace, float eps, int act, hipStream_t stream) {
-  constexpr int NT = kNormThreads;
-  const size_t lds = ((size_t)p.rows * p.s.slab + 2 * (p.s.slab / p.s.Cg)) * sizeof(float);
-  const dim3 grid((unsigned)((long long)p.s.N * p.s.chunks * p.s.slabs));
-  float *out = p.resident ? stats : workspace;
-#define FRCNN_NORM(NV, W)                                                                                                   \
-  {                                                                                                                         \
-    const int rc = ensure_dynamic_lds((const void *)norm_resident_kernel<T, VEC, NV, NT, W>, lds, "group_norm");            \
-    if (rc) return rc;                                                                                                      \
-    hipLaunchKernelGGL((norm_resident_kernel<T, VEC, NV, NT, W>), grid, dim3(NT), lds, stream, (const T *)x, (T *)y, gamma, \
-                       beta, out, p.s, eps, act);                                                                           \
-  }
+#define FRCNN_NORM(NV, W) return launch_resident<T, VEC, ONE, NV, W>(p, x, y, gamma, beta, W ? stats : workspace, eps, act, stream)
   if (p.resident) {
-    if (p.nv == 1) FRCNN_NORM(1, true) else if (p.nv == 2) FRCNN_NORM(2, true) else if (p.nv == 4) FRCNN_NORM(4, true)
-    else if (p.nv == 8) FRCNN_NORM(8, true) else FRCNN_NORM(16, true)
-    return check_launch("group_norm");
+    switch (p.nv) {
+      case 1: FRCNN_NORM(1, true);
+      case 4: FRCNN_NORM(4, true);
+      case 8: FRCNN_NORM(8, true);
+      case 16: FRCNN_NORM(16, true);
+    }
+    if constexpr (VEC > 1) switch (p.nv) {
+      case 2: FRCNN_NORM(2, true);
+      case 3: FRCNN_NORM(3, true);
+      case 5: FRCNN_NORM(5, true);
+      case 6: FRCNN_NORM(6, true);
+      case 7: FRCNN_NORM(7, true);
+      case 12: FRCNN_NORM(12, true);
+    }
+    return set_error(FRCNN_EUNSUPPORTED, "group_norm: no kernel for %d packs", p.nv);
   }
-  if (p.nv <= 2) FRCNN_NORM(2, false) else if (p.nv == 4) FRCNN_NORM(4, false) else if (p.nv == 8) FRCNN_NORM(8, false)
-  else FRCNN_NORM(16, false)
+  auto chunks = [&]() -> int {
+    if (p.nv <= 4) FRCNN_NORM(4, false);
+    FRCNN_NORM(8, false);
+  };
 #undef FRCNN_NORM
-  int rc = check_launch("group_norm");
+  int rc = chunks();
   if (rc) return rc;
+  const dim3 grid((unsigned)((long long)p.s.N * p.s.chunks * p.s.slabs));
   float *joined = stats ? stats : workspace + (size_t)p.s.N * p.s.chunks * p.s.G * 2;
   hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(((long long)p.s.N * p.s.G + 3) / 4)), dim3(256), 0, stream, workspace,
                      joined, p.s, eps);
   rc = check_launch("group_norm");
   if (rc) return rc;
-  hipLaunchKernelGGL((norm_apply_kernel<T, VEC, NT>), grid, dim3(NT), 0, stream, (const T *)x, (T *)y, gamma, beta, joined, p.s,
-                     act);
+  hipLaunchKernelGGL((norm_apply_kernel<T, VEC, ONE>), grid, dim3(p.threads), 0, stream, (const T *)x, (T *)y, gamma, beta, joined, p.s, act);
   return check_launch("group_norm");
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool ONE, int NV>
+static int launch_grad_resident(const NormPlan &p, const void *dy, const void *x, const float *gamma, const float *beta, const float *stats,
+                                void *dx, float *sums, int per, long long parts, int act, hipStream_t stream) {
+  const NormShape &s = p.s;
+  const size_t lds = (2 * (size_t)s.rows * s.slab + 2 * (s.slab / s.Cg) + s.slab) * sizeof(float);
+  const int rc = ensure_dynamic_lds((const void *)norm_grad_resident_kernel<T, VEC, ONE, NV>, lds, "group_norm_grad");
+  if (rc) return rc;
+  hipLaunchKernelGGL((norm_grad_resident_kernel<T, VEC, ONE, NV>), dim3((unsigned)(parts * s.slabs)), dim3(p.threads), lds, stream,
+                     (const T *)dy, (const T *)x, gamma, beta, stats, (T *)dx, sums, s, per, act);
+  return check_launch("group_norm_grad");
+}
+
+template <typename T, int VEC, bool ONE>
 static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, const float *gamma, const float *beta,
                             const float *stats, void *dx, float *dgamma, float *dbeta, float *workspace, int act,
                             hipStream_t stream) {
-  constexpr int NT = kNormThreads;
   const NormShape &s = p.s;
   long long parts;
   float *sums = workspace;
@@ -641,19 +740,24 @@ static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, co
   if (p.resident) {
     const int per = grad_images_per_group(p);
     parts = (s.N + per - 1) / per;
-    const size_t lds = (2 * (size_t)p.rows * s.slab + 2 * (s.slab / s.Cg) + s.slab) * sizeof(float);
-    const dim3 grid((unsigned)(parts * s.slabs));
-#define FRCNN_NORM_GRAD(NV)                                                                                                    \
-  {                                                                                                                            \
-    rc = ensure_dynamic_lds((const void *)norm_grad_resident_kernel<T, VEC, NV, NT>, lds, "group_norm_grad");                  \
-    if (rc) return rc;                                                                                                         \
-    hipLaunchKernelGGL((norm_grad_resident_kernel<T, VEC, NV, NT>), grid, dim3(NT), lds, stream, (const T *)dy, (const T *)x,  \
-                       gamma, beta, stats, (T *)dx, sums, s, per, act);                                                        \
-  }
-    if (p.nv == 1) FRCNN_NORM_GRAD(1) else if (p.nv == 2) FRCNN_NORM_GRAD(2) else if (p.nv == 4) FRCNN_NORM_GRAD(4)
-    else FRCNN_NORM_GRAD(8)
+    auto resident = [&]() -> int {
+#define FRCNN_NORM_GRAD(NV) return launch_grad_resident<T, VEC, ONE, NV>(p, dy, x, gamma, beta, stats, dx, sums, per, parts, act, stream)
+      switch (p.nv) {
+        case 1: FRCNN_NORM_GRAD(1);
+        case 4: FRCNN_NORM_GRAD(4);
+        case 8: FRCNN_NORM_GRAD(8);
+      }
+      if constexpr (VEC > 1) switch (p.nv) {
+        case 2: FRCNN_NORM_GRAD(2);
+        case 3: FRCNN_NORM_GRAD(3);
+        case 5: FRCNN_NORM_GRAD(5);
+        case 6: FRCNN_NORM_GRAD(6);
+        case 7: FRCNN_NORM_GRAD(7);
+      }
 #undef FRCNN_NORM_GRAD
-    rc = check_launch("group_norm_grad");
+      return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: no kernel for %d packs", p.nv);
+    };
+    rc = resident();
     if (rc) return rc;
   } else {
     parts = s.N;
@@ -661,10 +765,10 @@ static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, co
     float *chunk_sums = image_sums + (size_t)s.N * s.C * 2;
     sums = image_sums;
     const dim3 grid((unsigned)((long long)s.N * s.chunks * s.slabs));
-    const size_t lds = 2 * (size_t)p.rows * s.slab * sizeof(float);
-    rc = ensure_dynamic_lds((const void *)norm_grad_sums_kernel<T, VEC, NT>, lds, "group_norm_grad");
+    const size_t lds = 2 * (size_t)s.rows * s.slab * sizeof(float);
+    rc = ensure_dynamic_lds((const void *)norm_grad_sums_kernel<T, VEC, ONE>, lds, "group_norm_grad");
     if (rc) return rc;
-    hipLaunchKernelGGL((norm_grad_sums_kernel<T, VEC, NT>), grid, dim3(NT), lds, stream, (const T *)dy, (const T *)x, gamma, beta,
+    hipLaunchKernelGGL((norm_grad_sums_kernel<T, VEC, ONE>), grid, dim3(p.threads), lds, stream, (const T *)dy, (const T *)x, gamma, beta,
                        stats, chunk_sums, s, act);
     rc = check_launch("group_norm_grad");
     if (rc) return rc;
@@ -672,7 +776,7 @@ static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, co
                        expect, s);
     rc = check_launch("group_norm_grad");
     if (rc) return rc;
-    hipLaunchKernelGGL((norm_grad_apply_kernel<T, VEC, NT>), grid, dim3(NT), 0, stream, (const T *)dy, (const T *)x, gamma, beta,
+    hipLaunchKernelGGL((norm_grad_apply_kernel<T, VEC, ONE>), grid, dim3(p.threads), 0, stream, (const T *)dy, (const T *)x, gamma, beta,
                        stats, expect, (T *)dx, s, act);
     rc = check_launch("group_norm_grad");
     if (rc) return rc;
@@ -697,7 +801,7 @@ static int norm_check(const char *what, int type, int64_t N, int64_t S, int C, i
 static size_t norm_bytes(int N, int S, int C, int G, int elem, bool grad) {
   size_t most = 0;
   for (int aligned = 0; aligned < 2; ++aligned) {
-    const NormPlan p = norm_plan(N, S, C, G, elem, aligned != 0, grad ? kNormGradMost : kNormForwardMost);
+    const NormPlan p = norm_plan(N, S, C, G, elem, aligned != 0, grad);
     if (!p.vec) continue;
     size_t floats;
     if (!grad) {
@@ -733,9 +837,9 @@ int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int C, int G
   if (N == 0) return FRCNN_OK;
   FRCNN_REQUIRE(x && gamma && beta && y, "group_norm: null pointer");
   const int elem = (int)type_bytes(type);
-  FRCNN_REQUIRE(aligned_to(x, elem) && aligned_to(y, elem) && aligned_to(gamma, 4) && aligned_to(beta, 4) && aligned_to(stats, 4),
+  FRCNN_REQUIRE(aligned_to(x, elem) && aligned_to(y, elem) && aligned_to(gamma, 4) && aligned_to(beta, 4) && aligned_to(stats, 8),
                 "group_norm: misaligned pointer");
-  const NormPlan p = norm_plan((int)N, (int)S, C, G, elem, aligned_to(x, 16) && aligned_to(y, 16), kNormForwardMost);
+  const NormPlan p = norm_plan((int)N, (int)S, C, G, elem, aligned_to(x, 16) && aligned_to(y, 16), false);
   if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm: %d channels per group", C / G);
   if ((long long)N * p.s.chunks * p.s.slabs >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "group_norm: too many workgroups");
   const size_t need = frcnn_group_norm_workspace_bytes(type, N, S, C, G);
@@ -744,8 +848,9 @@ int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int C, int G
   hipStream_t st = (hipStream_t)stream;
   float *ws = (float *)workspace;
 #define FRCNN_NORM_T(T)                                                                                       \
-  (p.vec > 1 ? launch_norm<T, 16 / sizeof(T)>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st)       \
-             : launch_norm<T, 1>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st))
+  (p.vec == 1 ? launch_norm<T, 1, true>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st)                        \
+   : p.one    ? launch_norm<T, 16 / sizeof(T), true>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st)          \
+              : launch_norm<T, 16 / sizeof(T), false>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st))
   if (type == FRCNN_F32) return FRCNN_NORM_T(float);
   if (type == FRCNN_F16) return FRCNN_NORM_T(_Float16);
   return FRCNN_NORM_T(__bf16);
@@ -773,9 +878,9 @@ int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, in
   FRCNN_REQUIRE(dy && x && gamma && beta && stats && dx, "group_norm_grad: null pointer");
   const int elem = (int)type_bytes(type);
   FRCNN_REQUIRE(aligned_to(dy, elem) && aligned_to(x, elem) && aligned_to(dx, elem) && aligned_to(gamma, 4) && aligned_to(beta, 4) &&
-                    aligned_to(stats, 4),
+                    aligned_to(stats, 8),
                 "group_norm_grad: misaligned pointer");
-  const NormPlan p = norm_plan((int)N, (int)S, C, G, elem, aligned_to(x, 16) && aligned_to(dy, 16) && aligned_to(dx, 16), kNormGradMost);
+  const NormPlan p = norm_plan((int)N, (int)S, C, G, elem, aligned_to(x, 16) && aligned_to(dy, 16) && aligned_to(dx, 16), true);
   if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: %d channels per group", C / G);
   if ((long long)N * p.s.chunks * p.s.slabs >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: too many workgroups");
   const size_t need = frcnn_group_norm_grad_workspace_bytes(type, N, S, C, G);
@@ -783,8 +888,9 @@ int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, in
                 "group_norm_grad: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);
   float *ws = (float *)workspace;
 #define FRCNN_NORM_T(T)                                                                                                        \
-  (p.vec > 1 ? launch_norm_grad<T, 16 / sizeof(T)>(p, dy, x, gamma, beta, stats, dx, dgamma, dbeta, ws, activation, st)        \
-             : launch_norm_grad<T, 1>(p, dy, x, gamma, beta, stats, dx, dgamma, dbeta, ws, activation, st))
+  (p.vec == 1 ? launch_norm_grad<T, 1, true>(p, dy, x, gamma, beta, stats, dx, dgamma, dbeta, ws, activation, st)                      \
+   : p.one    ? launch_norm_grad<T, 16 / sizeof(T), true>(p, dy, x, gamma, beta, stats, dx, dgamma, dbeta, ws, activation, st)        \
+              : launch_norm_grad<T, 16 / sizeof(T), false>(p, dy, x, gamma, beta, stats, dx, dgamma, dbeta, ws, activation, st))
   if (type == FRCNN_F32) return FRCNN_NORM_T(float);
   if (type == FRCNN_F16) return FRCNN_NORM_T(_Float16);
   return FRCNN_NORM_T(__bf16);

@@ -164,7 +164,9 @@ __device__ __forceinline__ void with_output_type(const ProductArgs &p, F f) {
   else f((__bf16 *)nullptr);
 }
 
-// TM x TN tiles of 16 x 16 per workgroup; its W waves share the blocks of K and add their sums in LDS, in the waves' order.
+// TM x TN tiles of 16 x 16 per workgroup; its W waves share the blocks of K and add their sums in LDS, in the waves' order.  For
+// few rows, where the weights' way from memory is all there is: 116 MB for one row in 24 us, 4.8 TB/s.  More blocks in flight per
+// wave (two, four) gave nothing.
 template <int TM, int TN, int W, int MODE>
 __global__ __launch_bounds__(64 * W) void product_split_kernel(ProductArgs p, int tiles_n) {
   using S = Scale<MODE>;
@@ -499,7 +501,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_join_kernel(ProductArgs 
   const int n = tn * BN + (wave / WM) * NT * 16 + (f % NT) * 16 + (lane >> 4) * 4;
   const f32x4 *in = partial + ((long long)t * plan.pieces * (MT * NT) + f) * THREADS + threadIdx.x;
   f32x4 v = in[0];
-#pragma unroll 4
+#pragma unroll 8
   for (int i = 1; i < plan.pieces; ++i) v += in[(long long)i * (MT * NT * THREADS)];
   with_output_type(p, [&](auto *type) { store4<__remove_pointer(decltype(type))>(p, m, n, v); });
 }
@@ -553,7 +555,13 @@ static int best_form(int M, int N, int blocks, bool wide) {
   return best;
 }
 
-static bool use_tiles(int M, int N) { return M >= 64 && N >= 64; }
+// A workgroup of product_split_kernel streams 4 KB per 16 x 16 tile and block through the chip at about 7.5 TB/s.
+static bool use_tiles(int M, int N, int blocks, bool wide) {
+  if (M <= 16 || blocks == 0) return false;
+  const TileForm &f = kTileForms[best_form(M, N, blocks, wide)];
+  const double split_us = 4.0 + (double)((M + 15) / 16) * ((N + 15) / 16) * blocks * 5.5e-4;
+  return plan_us(f, tile_plan(f, M, N, blocks), blocks, wide) < split_us;
+}
 
 template <int MT, int NT, int WM, int WN, int PER_CU, int DB, int MODE>
 static int launch_tile(const ProductArgs &p, const TileForm &f, void *workspace, size_t workspace_bytes, hipStream_t s) {
@@ -599,9 +607,8 @@ static int launch_split(const ProductArgs &p, hipStream_t s) {
 
 template <int MODE>
 static int launch_product(const ProductArgs &p, void *workspace, size_t workspace_bytes, hipStream_t s) {
-  if (use_tiles(p.M, p.N)) return launch_tiles<MODE>(p, workspace, workspace_bytes, s);
-  if (p.M <= 16) return launch_split<1, 1, 16, MODE>(p, s);
-  return launch_split<4, 2, 4, MODE>(p, s);
+  if (use_tiles(p.M, p.N, p.blocks, MODE == kWideF32 || MODE == kWideE8M0)) return launch_tiles<MODE>(p, workspace, workspace_bytes, s);
+  return launch_split<1, 1, 16, MODE>(p, s);
 }
 
 }  // namespace frcnn
@@ -611,13 +618,13 @@ using namespace frcnn;
 extern "C" {
 
 size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K) {
-  if (K < 0 || !use_tiles(M, N)) return 0;
+  if (M < 1 || N < 1 || K < 1) return 0;
   const int blocks = (K + kQuantBlock - 1) / kQuantBlock;
   size_t most = 0;
   for (int wide = 0; wide < 2; ++wide) {  // the output's type decides
+    if (!use_tiles(M, N, blocks, wide != 0)) continue;
     const TileForm &f = kTileForms[best_form(M, N, blocks, wide != 0)];
-    const TilePlan t = tile_plan(f, M, N, blocks);
-    const size_t bytes = plan_bytes(f, t);
+    const size_t bytes = plan_bytes(f, tile_plan(f, M, N, blocks));
     if (bytes > most) most = bytes;
   }
   return most;

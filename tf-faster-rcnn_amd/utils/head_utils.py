@@ -24,6 +24,8 @@ _ACTIVATIONS = {None: 0, "linear": 0, "relu": 1, "swish": 2}
 
 def _operand(x: Any, name: str, types: Any = _TYPES, device: Optional[torch.device] = None) -> torch.Tensor:
     """``x`` as a device tensor (DLPack objects are imported zero-copy) of one of ``types``; its strides stay."""
+    if type(x) is torch.Tensor and x.is_cuda and x.dtype in types and (device is None or x.device == device):
+        return x
     if not isinstance(x, torch.Tensor):
         x = torch.from_dlpack(x) if hasattr(x, "__dlpack__") else torch.as_tensor(x)
     if x.dtype not in types:
@@ -40,8 +42,10 @@ def _activation(activation: Optional[str], known: Tuple[Optional[str], ...]) -> 
 
 
 def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
 def _leaves_of(*tensors: torch.Tensor) -> None:
@@ -67,8 +71,8 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 def _rows_of_16(t: torch.Tensor) -> torch.Tensor:
     """``t`` (rows, K) one byte an element with its rows at multiples of 16 bytes: as it is, or a padded copy."""
     rows, inner = t.shape
-    stride = t.stride(0) if rows > 1 else -(-inner // 16) * 16
-    if (inner <= 1 or t.stride(1) == 1) and stride >= inner and stride % 16 == 0 and t.data_ptr() % 16 == 0:
+    stride, step = t.stride()
+    if (step == 1 or inner <= 1) and (rows <= 1 or stride >= inner and stride % 16 == 0) and t.data_ptr() % 16 == 0:
         return t
     wide = torch.empty((rows, -(-inner // 16) * 16), dtype=t.dtype, device=t.device)[:, :inner]
     wide.view(torch.uint8).copy_(t.view(torch.uint8))
@@ -100,19 +104,19 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1,
     if scale_dtype not in _SCALE_TYPES:
         raise ValueError(f"scale_dtype must be one of {[str(t) for t in _SCALE_TYPES]}, got {scale_dtype}")
     device, lead, inner = x.device, x.shape[:-1], x.shape[-1]
-    rows = 1
-    for n in lead:
-        rows *= n
-    flat = x.reshape(rows, inner)
-    if inner > 1 and flat.stride(1) != 1 or rows > 1 and flat.stride(0) < inner:
+    flat = x if x.dim() == 2 else x.reshape(lead.numel(), inner)
+    rows = flat.shape[0]
+    stride, step = flat.stride()
+    if inner > 1 and step != 1 or rows > 1 and stride < inner:
         flat = flat.contiguous()
+        stride = inner
     across, up = -(-inner // BLOCK), -(-rows // block_rows)
     wide = -(-inner // 16) * 16
     q = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=device)
     scales = torch.empty((across, up), dtype=scale_dtype, device=device)
     with _lib.on_device(device):
-        _lib.check(_lib.lib().frcnn_quantize_blocks(_lib.ptr(flat), _TYPES[x.dtype], max(flat.stride(0), inner), rows, inner, block_rows,
-                                                    _lib.ptr(q), wide, _lib.ptr(scales), _SCALE_TYPES[scale_dtype], 1, up,
+        _lib.check(_lib.lib().frcnn_quantize_blocks(flat.data_ptr(), _TYPES[x.dtype], max(stride, inner), rows, inner, block_rows,
+                                                    q.data_ptr(), wide, scales.data_ptr(), _SCALE_TYPES[scale_dtype], 1, up,
                                                     _lib.stream_ptr(device)))
     q = q[:, :inner] if wide != inner else q
     return (q if len(lead) == 1 else q.unflatten(0, lead) if lead else q[0]), scales.t()
@@ -149,21 +153,18 @@ def scaled_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
         raise ValueError(f"out_dtype must be one of {[str(t) for t in _TYPES]}, got {out_dtype}")
     if a.dim() < 1 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
         raise ValueError(f"a must be (..., K) and b (N, K), got {tuple(a.shape)} and {tuple(b.shape)}")
-    lead, inner, units = a.shape[:-1], a.shape[-1], b.shape[0]
-    rows = 1
-    for n in lead:
-        rows *= n
-    across = -(-inner // BLOCK)
-    if tuple(a_scales.shape) != (rows, across):
+    lead, (units, inner) = a.shape[:-1], b.shape
+    if len(lead) != 1:
+        a = a.reshape(lead.numel(), inner)
+    rows, across, up = a.shape[0], -(-inner // BLOCK), -(-units // BLOCK)
+    if a_scales.shape != (rows, across):
         raise ValueError(f"a_scales must be ({rows}, {across}), got {tuple(a_scales.shape)}")
-    if tuple(b_scales.shape) != (-(-units // BLOCK), across):
-        raise ValueError(f"b_scales must be ({-(-units // BLOCK)}, {across}), got {tuple(b_scales.shape)}")
+    if b_scales.shape != (up, across):
+        raise ValueError(f"b_scales must be ({up}, {across}), got {tuple(b_scales.shape)}")
     if a_scales.dtype != b_scales.dtype:
         raise ValueError(f"a_scales and b_scales must be of one type, got {a_scales.dtype} and {b_scales.dtype}")
-    if bias is not None and tuple(bias.shape) != (units,):
+    if bias is not None and bias.shape != (units,):
         raise ValueError(f"bias must be ({units},), got {tuple(bias.shape)}")
-    if len(lead) != 1:
-        a = a.reshape(rows, inner)
     a, b = _rows_of_16(a), _rows_of_16(b)
     out = torch.empty((rows, units), dtype=out_dtype, device=device)
     lib = _lib.lib()
@@ -171,21 +172,17 @@ def scaled_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
     nbytes = lib.frcnn_scaled_matmul_workspace_bytes(rows, units, inner)
     ws = _workspace(nbytes, device) if nbytes else None
     with _lib.on_device(device):
-        _lib.check(lib.frcnn_scaled_matmul(_lib.ptr(a), a.stride(0) if rows > 1 else pad, _lib.ptr(a_scales), a_scales.stride(0),
-                                           a_scales.stride(1), _lib.ptr(b), b.stride(0) if units > 1 else pad, _lib.ptr(b_scales),
-                                           b_scales.stride(0), b_scales.stride(1), _SCALE_TYPES[a_scales.dtype], _lib.ptr(bias), act,
-                                           rows, units, inner, _lib.ptr(out), _TYPES[out_dtype], units, _lib.ptr(ws), nbytes,
-                                           _lib.stream_ptr(device)))
+        _lib.check(lib.frcnn_scaled_matmul(a.data_ptr(), a.stride(0) if rows > 1 else pad, a_scales.data_ptr(), *a_scales.stride(),
+                                           b.data_ptr(), b.stride(0) if units > 1 else pad, b_scales.data_ptr(), *b_scales.stride(),
+                                           _SCALE_TYPES[a_scales.dtype], _lib.ptr(bias), act, rows, units, inner, out.data_ptr(),
+                                           _TYPES[out_dtype], units, _lib.ptr(ws), nbytes, _lib.stream_ptr(device)))
     return out if len(lead) == 1 else out.view(*lead, units)
 
 
 def _norm_shape(x: torch.Tensor, groups: int) -> Tuple[int, int, int]:
     if x.dim() < 2:
         raise ValueError(f"x must be (batch, ..., channels), got {tuple(x.shape)}")
-    batch, channels = x.shape[0], x.shape[-1]
-    positions = 1
-    for n in x.shape[1:-1]:
-        positions *= n
+    batch, channels, positions = x.shape[0], x.shape[-1], x.shape[1:-1].numel()
     if groups < 1 or channels < 1 or channels % groups:
         raise ValueError(f"{channels} channels are not a multiple of {groups} groups")
     if positions < 1:
@@ -195,7 +192,7 @@ def _norm_shape(x: torch.Tensor, groups: int) -> Tuple[int, int, int]:
 
 def _parameters(gamma: Any, beta: Any, channels: int, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
     gamma, beta = _lib.device_tensor(gamma, torch.float32, device), _lib.device_tensor(beta, torch.float32, device)
-    if tuple(gamma.shape) != (channels,) or tuple(beta.shape) != (channels,):
+    if gamma.shape != (channels,) or beta.shape != (channels,):
         raise ValueError(f"gamma and beta must be ({channels},), got {tuple(gamma.shape)} and {tuple(beta.shape)}")
     return gamma, beta
 
@@ -204,7 +201,7 @@ def _norm_forward(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, grou
                   want_stats: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     batch, positions, channels = _norm_shape(x, groups)
     device = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    y = torch.empty_like(x)
     stats = torch.empty((batch, groups, 2), dtype=torch.float32, device=device) if want_stats else None
     lib = _lib.lib()
     nbytes = lib.frcnn_group_norm_workspace_bytes(_TYPES[x.dtype], batch, positions, channels, groups)
@@ -221,9 +218,8 @@ def _norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, beta:
     groups = stats.shape[1]
     batch, positions, channels = _norm_shape(x, groups)
     device = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-    grads = torch.empty((2, channels), dtype=torch.float32, device=device)
-    dgamma, dbeta = grads.unbind(0)
+    dx = torch.empty_like(x)
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
     lib = _lib.lib()
     nbytes = lib.frcnn_group_norm_grad_workspace_bytes(_TYPES[x.dtype], batch, positions, channels, groups)
     ws = _workspace(nbytes, device) if nbytes else None
@@ -297,6 +293,8 @@ def group_norm_gradients(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor,
     stats = _lib.device_tensor(stats, torch.float32, device)
     if stats.dim() != 3 or stats.shape[0] != x.shape[0] or stats.shape[2] != 2:
         raise ValueError(f"stats must be ({x.shape[0]}, groups, 2), got {tuple(stats.shape)}")
+    if stats.data_ptr() % 8:
+        stats = stats.clone()
     act = _activation(activation, (None, "linear", "relu", "swish"))
     _, _, channels = _norm_shape(x, stats.shape[1])
     gamma, beta = _parameters(gamma, beta, channels, device)
@@ -305,7 +303,7 @@ def group_norm_gradients(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor,
 
 
 def _dropout(x: torch.Tensor, rate: float, seed: int, offset: int, state: Optional[torch.Tensor]) -> torch.Tensor:
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     with _lib.on_device(x.device):
         _lib.check(_lib.lib().frcnn_dropout(_lib.ptr(x), _lib.ptr(y), _TYPES[x.dtype], x.numel(), rate, seed, offset, _lib.ptr(state),
                                             _lib.stream_ptr(x.device)))
