@@ -10,8 +10,9 @@
 // data is read once.  Where a slab of one image does not fit a workgroup's registers the positions are cut into chunks:
 // statistics per chunk, joined in a fixed order (Chan, Golub and LeVeque's update), then a second pass over the data.
 //
-// A thread owns one pack of channels (a column) and walks the positions.  Sums are kept per channel -- a pack may straddle
-// groups -- added over the workgroup's rows in LDS by halving, then over the channels of each group by lanes of one wave.
+// A thread owns one pack of channels (a column) and walks the positions.  Where a pack lies in one group a thread hands over
+// one number per sum, and lanes of one wave add a group's; where it straddles groups the channels' sums are added over the
+// workgroup's rows in LDS by halving first.
 // No atomics: results do not depend on the order in which workgroups run.
 #include "head_common.hpp"
 
@@ -89,20 +90,28 @@ __device__ __forceinline__ void rows_to_first(float *red, int rows, int slab, in
   __syncthreads();
 }
 
-// out[g] = sum of weight(c) * chan[c] over the group's channels; P lanes (a power of two <= 64) per group.
-template <typename F>
-__device__ __forceinline__ void groups_of(int groups, int Cg, int threads, F value, float *out) {
+// out[k][g] = the sum of value(k, g, i) over i < count, for the K sums at once; P lanes (a power of two <= 64) per group.
+template <int K, typename F>
+__device__ __forceinline__ void groups_of(int groups, int count, F value, float *out, int stride) {
   int P = 1;
-  while (P < Cg && P < 64) P <<= 1;
-  const int per = threads / P;
+  while (P < count && P < 64) P <<= 1;
+  const int per = (int)blockDim.x / P;
   const int sub = threadIdx.x & (P - 1), first = threadIdx.x / P;
   for (int base = 0; base < groups; base += per) {
     const int g = base + first;
-    float s = 0.0f;
+    float s[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = 0.0f;
     if (g < groups)
-      for (int c = sub; c < Cg; c += P) s += value(g * Cg + c);
-    for (int d = P >> 1; d > 0; d >>= 1) s += __shfl_xor(s, d);
-    if (g < groups && sub == 0) out[g] = s;
+      for (int i = sub; i < count; i += P)
+#pragma unroll
+        for (int k = 0; k < K; ++k) s[k] += value(k, g, i);
+    for (int d = P >> 1; d > 0; d >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[k] += __shfl_xor(s[k], d);
+    if (g < groups && sub == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) out[k * stride + g] = s[k];
   }
   __syncthreads();
 }
@@ -128,6 +137,51 @@ struct Column {  // a thread's place in the slab
     active = row < rows && col < width;
   }
 };
+
+// out[k][g] = the sums of v[k] over the group's channels and all rows.  With one group per pack a thread hands over one number
+// per sum; otherwise the channels are added over the rows first.
+template <int VEC, bool ONE, int K>
+__device__ __forceinline__ void group_sums(const NormShape &s, const Column<VEC> &me, float *red, float (&v)[K][VEC], float *out) {
+  const int groups = me.width / s.Cg, stride = s.slab / s.Cg;
+  if constexpr (ONE) {
+    const int vc = s.slab / VEC, packs = s.Cg / VEC;
+    if (me.active)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float t = v[k][0];
+#pragma unroll
+        for (int e = 1; e < VEC; ++e) t += v[k][e];
+        red[(k * s.rows + me.row) * vc + me.col / VEC] = t;
+      }
+    __syncthreads();
+    if (packs == 1)
+      groups_of<K>(groups, s.rows, [&](int k, int g, int i) { return red[(k * s.rows + i) * vc + g]; }, out, stride);
+    else
+      groups_of<K>(groups, s.rows * packs, [&](int k, int g, int i) {
+        const int row = i / packs;
+        return red[(k * s.rows + row) * vc + g * packs + i - row * packs];
+      }, out, stride);
+  } else {
+    rows_to_first<VEC, K>(red, s.rows, s.slab, me.row, me.col, me.active, v);
+    const int plane = s.rows * s.slab;
+    groups_of<K>(groups, s.Cg, [&](int k, int g, int i) { return red[k * plane + g * s.Cg + i]; }, out, stride);
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_parameters(const float *p, float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    f[0] = *p;
+  } else {
+    typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // a four-word load needs four-byte alignment
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const f32x4 v = *reinterpret_cast<const f32x4_any *>(p + 4 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[4 * i + e] = v[e];
+    }
+  }
+}
 
 // ---- forward, a slab of one image (or one chunk of it) in registers --------------------------------------------------------
 // WRITE: apply and write y (the whole image is here: chunks == 1).  Otherwise only the chunk's mean and the sum of its
@@ -169,9 +223,8 @@ __global__ __launch_bounds__(1024) void norm_resident_kernel(const T *__restrict
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[0][e] += f[e];  // rows beyond the end hold zeros
   }
-  rows_to_first<VEC, 1>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
+  group_sums<VEC, ONE, 1>(s, me, red, sum, gsum);
   const float inv = 1.0f / ((float)count * (float)s.Cg);
-  groups_of(groups, s.Cg, (int)blockDim.x, [&](int c) { return red[c]; }, gsum);
 
   float mean[Gs::N];
 #pragma unroll
@@ -190,8 +243,7 @@ __global__ __launch_bounds__(1024) void norm_resident_kernel(const T *__restrict
       }
     }
   }
-  rows_to_first<VEC, 1>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
-  groups_of(groups, s.Cg, (int)blockDim.x, [&](int c) { return red[c]; }, grstd);
+  group_sums<VEC, ONE, 1>(s, me, red, sum, grstd);
 
   const int g0 = slab_index * s.slab / s.Cg;
   if constexpr (!WRITE) {
@@ -212,11 +264,10 @@ __global__ __launch_bounds__(1024) void norm_resident_kernel(const T *__restrict
     float a[VEC], b[VEC], rstd[Gs::N];
 #pragma unroll
     for (int e = 0; e < Gs::N; ++e) rstd[e] = 1.0f / __builtin_sqrtf(__builtin_fmaf(grstd[group[e]], inv, eps));
+    load_parameters(gamma + c0, a);
+    load_parameters(beta + c0, b);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      a[e] = gamma[c0 + e] * rstd[Gs::of(e)];
-      b[e] = beta[c0 + e];
-    }
+    for (int e = 0; e < VEC; ++e) a[e] *= rstd[Gs::of(e)];
     with_activation(act, [&](auto which) {
       constexpr int ACT = decltype(which)::value;
 #pragma unroll
@@ -289,11 +340,10 @@ __global__ __launch_bounds__(1024) void norm_apply_kernel(const T *__restrict__ 
     mean[e] = st.x;
     rstd[e] = st.y;
   }
+  load_parameters(gamma + c0, a);
+  load_parameters(beta + c0, b);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    a[e] = gamma[c0 + e] * rstd[Gs::of(e)];
-    b[e] = beta[c0 + e];
-  }
+  for (int e = 0; e < VEC; ++e) a[e] *= rstd[Gs::of(e)];
   with_activation(act, [&](auto which) {
     constexpr int ACT = decltype(which)::value;
 #pragma unroll 4
@@ -313,11 +363,8 @@ struct GradCoefficients {
   using Gs = Groups<VEC, ONE>;
   float mean[Gs::N], rstd[Gs::N], gamma[VEC], beta[VEC];
   __device__ __forceinline__ void parameters(const float *__restrict__ g, const float *__restrict__ b, int c0) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      gamma[e] = g[c0 + e];
-      beta[e] = b[c0 + e];
-    }
+    load_parameters(g + c0, gamma);
+    load_parameters(b + c0, beta);
   }
   __device__ __forceinline__ void statistics(const float *__restrict__ stats, const NormShape &s, int n, int c0) {
 #pragma unroll
@@ -350,10 +397,7 @@ __global__ __launch_bounds__(512) void norm_grad_resident_kernel(const T *__rest
   const int part = (int)(blockIdx.x / (unsigned)s.slabs);
   const Column<VEC> me(s, slab_index);
   const int c0 = slab_index * s.slab + me.col;
-  const int groups = me.width / s.Cg;
-  float *red = lds, *first = lds + 2 * me.rows * s.slab, *second = first + s.slab / s.Cg, *weight = second + s.slab / s.Cg;
-  const int plane = me.rows * s.slab;
-  for (int c = threadIdx.x; c < me.width; c += blockDim.x) weight[c] = gamma[slab_index * s.slab + c];
+  float *red = lds, *first = lds + 2 * me.rows * s.slab, *second = first + s.slab / s.Cg;
   int group[Gs::N];
 #pragma unroll
   for (int e = 0; e < Gs::N; ++e) group[e] = me.active ? (me.col + e) / s.Cg : 0;
@@ -397,15 +441,14 @@ __global__ __launch_bounds__(512) void norm_grad_resident_kernel(const T *__rest
         }
       }
     });
-    rows_to_first<VEC, 2>(red, me.rows, s.slab, me.row, me.col, me.active, sum);
-    if (me.active && me.row == 0)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        total[0][e] += sum[0][e];
-        total[1][e] += sum[1][e];
-      }
-    groups_of(groups, s.Cg, (int)blockDim.x, [&](int c) { return red[c] * weight[c]; }, first);
-    groups_of(groups, s.Cg, (int)blockDim.x, [&](int c) { return red[plane + c] * weight[c]; }, second);
+    for (int e = 0; e < VEC; ++e) {
+      total[0][e] += sum[0][e];
+      total[1][e] += sum[1][e];
+      sum[0][e] *= k.gamma[e];
+      sum[1][e] *= k.gamma[e];
+    }
+    group_sums<VEC, ONE, 2>(s, me, red, sum, first);
     if (me.active) {
       float d1[Gs::N], d2[Gs::N];
 #pragma unroll
@@ -427,6 +470,7 @@ __global__ __launch_bounds__(512) void norm_grad_resident_kernel(const T *__rest
     }
     __syncthreads();  // red, first and second are free for the next image
   }
+  rows_to_first<VEC, 2>(red, me.rows, s.slab, me.row, me.col, me.active, total);
   if (me.active && me.row == 0)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -600,8 +644,8 @@ struct NormPlan {
 
 static int gcd_int(int a, int b) { return b ? gcd_int(b, a % b) : a; }
 
-// Threads for a slab of `columns` packs of S positions, `most` packs per thread: the least idle lanes, about six packs each (bytes
-// in flight against waves).  0: none fits.
+// Threads for a slab of `columns` packs of S positions, `most` packs per thread: the least idle lanes, and near four packs each
+// (bytes in flight against registers, that is waves).  0: none fits.
 static int norm_threads(int columns, int S, int most, int limit) {
   int best = 0;
   float least = 0;
@@ -610,14 +654,14 @@ static int norm_threads(int columns, int S, int most, int limit) {
     if (!rows) continue;
     const int need = (S + rows - 1) / rows;
     if (need > most) continue;
-    const float cost = (float)t * need / ((float)columns * S) + 0.02f * (need > 6 ? need - 6 : 6 - need);
+    const float cost = (float)t * need / ((float)columns * S) + 0.02f * (need > 4 ? need - 4 : 4 - need);
     if (!best || cost < least) best = t, least = cost;
   }
   return best;
 }
 
-// Whole images per workgroup where a slab's packs fit its registers, chunks of positions otherwise.  grad: two tensors are held,
-// in up to 512 threads of 8 packs; the forward pass holds one, in up to 512 threads of 8 or 1024 of 16.
+// Whole images per workgroup where a slab's packs fit its registers, chunks of positions otherwise.  grad: x and dz are held, in up
+// to 512 threads of 8 packs; the forward pass holds x, in up to 1024 threads of 16.
 static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, bool grad) {
   NormPlan p = {};
   p.s.N = N, p.s.S = S, p.s.C = C, p.s.G = G, p.s.Cg = C / G;
@@ -633,17 +677,30 @@ static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, bo
   const long long units = C / unit;
   long long widest = kNormColumns * (long long)vec / unit;  // units per slab
   if (widest > units) widest = units;
-  auto threads = [&](long long k) {
-    const int t = norm_threads((int)(k * unit / vec), S, 8, 512);
-    return t || grad ? t : norm_threads((int)(k * unit / vec), S, 16, 1024);
-  };
+  auto threads = [&](long long k, int most, int limit) { return norm_threads((int)(k * unit / vec), S, most, limit); };
+  // Packs per thread and threads, in the order in which they are tried.  Small workgroups, of which two or more share a CU and
+  // overlap one's loads with another's sums, before large ones: (6000, 49, 512) bf16 forward 125 us with 256 threads and 142 with
+  // 448, its gradients 207 and 229; not in
+  // fp32, where a narrower slab's shorter rows cost more: (4800, 49, 576) forward 222 us against 204.
+  const int choices[3][2] = {{8, elem == 2 ? 256 : 0}, {8, 512}, {16, grad ? 0 : 1024}};
+  int most = 0, limit = 0;
   // the widest slab that fits; narrower ones while the chip is not full and a row is still a line
   long long k = widest;
-  while (k > 1 && !threads(k)) k = (k + 1) / 2;
-  p.resident = threads(k) && (k == units || k * unit * elem >= kNormLine);
+  auto narrow_enough = [&]() {
+    for (k = widest;; k = (k + 1) / 2) {
+      if (threads(k, most, limit)) return k == units || k * unit * elem >= kNormLine;
+      if (k == 1) return false;
+    }
+  };
+  for (const auto &c : choices) {
+    most = c[0], limit = c[1];
+    p.resident = narrow_enough();
+    if (p.resident) break;
+  }
   if (p.resident) {
-    while (k > 1 && (long long)N * ((units + k - 1) / k) < 1024 && (k + 1) / 2 * unit * elem >= kNormLine && threads((k + 1) / 2)) k = (k + 1) / 2;
-    p.threads = threads(k);
+    while (k > 1 && (long long)N * ((units + k - 1) / k) < 1024 && (k + 1) / 2 * unit * elem >= kNormLine && threads((k + 1) / 2, most, limit))
+      k = (k + 1) / 2;
+    p.threads = threads(k, most, limit);
     p.s.chunk = S;
   } else {
     k = widest;
@@ -654,7 +711,7 @@ static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, bo
   p.s.rows = p.threads / (p.s.slab / vec);
   if (!p.resident) {
     int per = 8;  // packs per thread and chunk; fewer while the chip is not full, at least four for a chunk's fixed costs
-    while (per > 4 && (long long)N * p.s.slabs * ((S + p.s.rows * per - 1) / (p.s.rows * per)) < 512) per /= 2;
+    while (per > 4 && (long long)N * p.s.slabs * ((S + p.s.rows * per - 1) / (p.s.rows * per)) < 400) per /= 2;
     p.s.chunk = p.s.rows * per;
   }
   p.s.chunks = (S + p.s.chunk - 1) / p.s.chunk;
@@ -721,7 +778,7 @@ template <typename T, int VEC, bool ONE, int NV>
 static int launch_grad_resident(const NormPlan &p, const void *dy, const void *x, const float *gamma, const float *beta, const float *stats,
                                 void *dx, float *sums, int per, long long parts, int act, hipStream_t stream) {
   const NormShape &s = p.s;
-  const size_t lds = (2 * (size_t)s.rows * s.slab + 2 * (s.slab / s.Cg) + s.slab) * sizeof(float);
+  const size_t lds = (2 * (size_t)s.rows * s.slab + 2 * (s.slab / s.Cg)) * sizeof(float);
   const int rc = ensure_dynamic_lds((const void *)norm_grad_resident_kernel<T, VEC, ONE, NV>, lds, "group_norm_grad");
   if (rc) return rc;
   hipLaunchKernelGGL((norm_grad_resident_kernel<T, VEC, ONE, NV>), dim3((unsigned)(parts * s.slabs)), dim3(p.threads), lds, stream,
