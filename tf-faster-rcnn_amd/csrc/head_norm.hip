@@ -10,9 +10,8 @@
 // data is read once.  Where a slab of one image does not fit a workgroup's registers the positions are cut into chunks:
 // statistics per chunk, joined in a fixed order (Chan, Golub and LeVeque's update), then a second pass over the data.
 //
-// A thread owns one pack of channels (a column) and walks the positions.  Where a pack lies in one group a thread hands over
-// one number per sum, and lanes of one wave add a group's; where it straddles groups the channels' sums are added over the
-// workgroup's rows in LDS by halving first.
+// A thread owns one pack of channels (a column) and walks the positions.  It hands over one number per sum where its pack lies in
+// one group, one per channel where it straddles groups; lanes of one wave add a group's.
 // No atomics: results do not depend on the order in which workgroups run.
 #include "head_common.hpp"
 
@@ -90,11 +89,15 @@ __device__ __forceinline__ void rows_to_first(float *red, int rows, int slab, in
   __syncthreads();
 }
 
-// out[k][g] = the sum of value(k, g, i) over i < count, for the K sums at once; P lanes (a power of two <= 64) per group.
-template <int K, typename F>
-__device__ __forceinline__ void groups_of(int groups, int count, F value, float *out, int stride) {
+// out[k][g] = the sum of red[k][row][g * width + c] over the rows and c < width, for K sums (planes of red) at once.  P lanes (a
+// power of two <= 64) per group, along the longer of the two directions.
+template <int K>
+__device__ __forceinline__ void groups_of(const float *red, int rows, int columns, int groups, int width, float *out, int stride) {
+  const bool down = rows >= width;
+  const int along = down ? rows : width, across = down ? width : rows;
+  const int step_along = down ? columns : 1, step_across = down ? 1 : columns;
   int P = 1;
-  while (P < count && P < 64) P <<= 1;
+  while (P < along && P < 64) P <<= 1;
   const int per = (int)blockDim.x / P;
   const int sub = threadIdx.x & (P - 1), first = threadIdx.x / P;
   for (int base = 0; base < groups; base += per) {
@@ -103,9 +106,12 @@ __device__ __forceinline__ void groups_of(int groups, int count, F value, float 
 #pragma unroll
     for (int k = 0; k < K; ++k) s[k] = 0.0f;
     if (g < groups)
-      for (int i = sub; i < count; i += P)
+      for (int i = sub; i < along; i += P) {
+        const float *at = red + g * width + i * step_along;
+        for (int j = 0; j < across; ++j)
 #pragma unroll
-        for (int k = 0; k < K; ++k) s[k] += value(k, g, i);
+          for (int k = 0; k < K; ++k) s[k] += at[k * rows * columns + j * step_across];
+      }
     for (int d = P >> 1; d > 0; d >>= 1)
 #pragma unroll
       for (int k = 0; k < K; ++k) s[k] += __shfl_xor(s[k], d);
@@ -139,33 +145,27 @@ struct Column {  // a thread's place in the slab
 };
 
 // out[k][g] = the sums of v[k] over the group's channels and all rows.  With one group per pack a thread hands over one number
-// per sum; otherwise the channels are added over the rows first.
+// per sum, otherwise one per channel.
 template <int VEC, bool ONE, int K>
-__device__ __forceinline__ void group_sums(const NormShape &s, const Column<VEC> &me, float *red, float (&v)[K][VEC], float *out) {
+__device__ __forceinline__ void group_sums(const NormShape &s, const Column<VEC> &me, float *red, const float (&v)[K][VEC], float *out) {
   const int groups = me.width / s.Cg, stride = s.slab / s.Cg;
-  if constexpr (ONE) {
-    const int vc = s.slab / VEC, packs = s.Cg / VEC;
-    if (me.active)
+  const int columns = ONE ? s.slab / VEC : s.slab;
+  if (me.active)
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
+    for (int k = 0; k < K; ++k) {
+      float *at = red + (k * s.rows + me.row) * columns + (ONE ? me.col / VEC : me.col);
+      if constexpr (ONE) {
         float t = v[k][0];
 #pragma unroll
         for (int e = 1; e < VEC; ++e) t += v[k][e];
-        red[(k * s.rows + me.row) * vc + me.col / VEC] = t;
+        *at = t;
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) at[e] = v[k][e];
       }
-    __syncthreads();
-    if (packs == 1)
-      groups_of<K>(groups, s.rows, [&](int k, int g, int i) { return red[(k * s.rows + i) * vc + g]; }, out, stride);
-    else
-      groups_of<K>(groups, s.rows * packs, [&](int k, int g, int i) {
-        const int row = i / packs;
-        return red[(k * s.rows + row) * vc + g * packs + i - row * packs];
-      }, out, stride);
-  } else {
-    rows_to_first<VEC, K>(red, s.rows, s.slab, me.row, me.col, me.active, v);
-    const int plane = s.rows * s.slab;
-    groups_of<K>(groups, s.Cg, [&](int k, int g, int i) { return red[k * plane + g * s.Cg + i]; }, out, stride);
-  }
+    }
+  __syncthreads();
+  groups_of<K>(red, s.rows, columns, groups, ONE ? s.Cg / VEC : s.Cg, out, stride);
 }
 
 template <int VEC>
