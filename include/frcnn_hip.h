@@ -266,8 +266,8 @@ int frcnn_roi_delta(const float *rois, const float *gt_boxes, const int32_t *gt_
 #define FRCNN_ACT_SWISH 2 /* z / (1 + exp(-z)) */
 
 /* Rows of x (rows, K; row stride ldx elements) to OCP e4m3 with one scale per block of block_rows (1 or 128) x 128 elements:
- * scale = max(amax / 448, 2^-126) over the block's finite values, 1 where they are all zero (FRCNN_SCALE_E8M0: the smallest
- * power of two that is not below amax / 448, 2^-126 at least); q = x / scale rounded to nearest even.  NaN and infinities
+ * scale = max(amax * fl(1 / 448), 2^-126) over the block's finite values, 1 where they are all zero (FRCNN_SCALE_E8M0: the
+ * smallest power of two that is not below amax / 448, 2^-126 at least); q = x / scale rounded to nearest even.  NaN and infinities
  * become e4m3's NaN.  q (rows, K) has the row stride ldq, a multiple of 16, and starts at a multiple of 16 bytes; of each row
  * the bytes up to the next multiple of 16 are written (zeros behind K).  Scale (r / block_rows, kb) is written to
  * scales[(r / block_rows) * scale_row_stride + kb * scale_block_stride] (strides in elements). */

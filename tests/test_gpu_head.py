@@ -38,8 +38,9 @@ def e4m3_nearest(v):
 
 
 def quantized(x, block_rows, scale_dtype):
-    """(values, scales) by the definition.  The scale and the quotient are fp32 operations of the definition, each correctly
-    rounded: 64-bit division of fp32 numbers rounded to fp32 is the correctly rounded fp32 quotient (53 >= 2 * 24 + 2)."""
+    """(values, scales) by the definition.  The scale's product and the quotient are fp32 operations of the definition, each
+    correctly rounded: in 64 bits the product of two fp32 numbers is exact, and the quotient rounded to fp32 is the correctly
+    rounded fp32 quotient (53 >= 2 * 24 + 2)."""
     rows, inner = x.shape
     up, across = -(-rows // block_rows), -(-inner // 128)
     v = torch.zeros((up * block_rows, across * 128), dtype=torch.float64, device=x.device)
@@ -47,7 +48,7 @@ def quantized(x, block_rows, scale_dtype):
     v = v.view(up, block_rows, across, 128)
     amax = torch.where(torch.isfinite(v), v.abs(), 0.0).amax((1, 3))
     if scale_dtype == F32:
-        s = (amax / 448).float().double().clamp_min(2.0 ** -126)
+        s = (amax * float(np.float32(1 / 448))).float().double().clamp_min(2.0 ** -126)
     else:
         f, e = torch.frexp(amax)
         e = (e - 9 + (f > 0.875).int()).clamp_min(-126)

@@ -1,7 +1,8 @@
 // head_quantize.hip -- rows to e4m3 with one scale per block of 128 elements.
 //
-// scale = max(amax / 448, 2^-126) over the block's finite values (1 where they are all zero), or the smallest power of two
-// that is not below amax / 448; q = x / scale rounded to the nearest e4m3, ties to even.  NaN and infinities become e4m3's
+// scale = max(amax * (1 / 448), 2^-126) over the block's finite values (1 where they are all zero; 1 / 448 rounded to fp32, the
+// product too), or the smallest power of two that is not below amax / 448; q = x / scale, the correctly rounded fp32 quotient,
+// rounded to the nearest e4m3, ties to even.  NaN and infinities become e4m3's
 // NaN and leave the scale to their finite neighbours.  Blocks are 1 x 128 (activations) or 128 x 128 (weights).
 //
 // Bound by memory: 2 or 4 bytes read and one written per element.  16 lanes hold a block's row, 8 elements each.
@@ -20,7 +21,7 @@ __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d
 __device__ __forceinline__ float block_scale(float amax, bool power_of_two) {
   if (amax == 0.0f) return 1.0f;
   if (!power_of_two) {
-    const float s = amax / kE4M3Max;
+    const float s = amax * (1.0f / kE4M3Max);
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;
   }
   // amax = 1.f * 2^e: amax / 448 = (1.f / 1.75) * 2^(e - 8)

@@ -83,7 +83,7 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1,
                     scale_dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows to ``torch.float8_e4m3fn`` with one scale per block of ``block_rows`` x 128 elements.
 
-    ``scale = max(amax / 448, 2^-126)`` over the block's finite values (1 where they are all zero); with ``scale_dtype``
+    ``scale = max(amax * (1 / 448), 2^-126)`` in fp32 over the block's finite values (1 where they are all zero); with ``scale_dtype``
     ``torch.float8_e8m0fnu`` the smallest power of two that is not below ``amax / 448``.  ``q = x / scale`` to nearest even.
     NaN and infinities become NaN and leave the scale to their finite neighbours.
 
@@ -111,15 +111,16 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1,
         flat = flat.contiguous()
         stride = inner
     across, up = -(-inner // BLOCK), -(-rows // block_rows)
-    wide = -(-inner // 16) * 16
+    # rows of a block or more start at whole lines of memory: the product reads them a line at a time
+    wide = -(-inner // BLOCK) * BLOCK if inner >= BLOCK else -(-inner // 16) * 16
     q = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty((across, up), dtype=scale_dtype, device=device)
+    scales = torch.empty_strided((up, across), (1, up), dtype=scale_dtype, device=device)
     with _lib.on_device(device):
         _lib.check(_lib.lib().frcnn_quantize_blocks(flat.data_ptr(), _TYPES[x.dtype], max(stride, inner), rows, inner, block_rows,
                                                     q.data_ptr(), wide, scales.data_ptr(), _SCALE_TYPES[scale_dtype], 1, up,
                                                     _lib.stream_ptr(device)))
     q = q[:, :inner] if wide != inner else q
-    return (q if len(lead) == 1 else q.unflatten(0, lead) if lead else q[0]), scales.t()
+    return (q if len(lead) == 1 else q.unflatten(0, lead) if lead else q[0]), scales
 
 
 def scaled_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
