@@ -217,13 +217,30 @@ def test_scaled_matmul_poisoned_rows_stay_alone(head, rows, out_dtype):
     assert torch.equal(y[~bad], clean[~bad].clamp_min(0))
 
 
-def test_scaled_matmul_e8m0_special_scales(head):
-    a, sa, b, sb = operands(4, 20, 256, E8M0, 2)
+@pytest.mark.parametrize("rows", [4, 200])
+def test_scaled_matmul_e8m0_special_scales(head, rows):
+    a, sa, b, sb = operands(rows, 200, 256, E8M0, 2)
     s = sa.view(torch.uint8)
     s[1, 0] = 255  # NaN
+    keep = torch.arange(rows, device="cuda") != 1
     for out_dtype in (F32, BF16):
         y = head.scaled_matmul(a, sa, b, sb, out_dtype=out_dtype)
-        assert torch.isnan(y[1]).all() and torch.isfinite(y[[0, 2, 3]]).all()
+        assert torch.isnan(y[1]).all() and torch.isfinite(y[keep]).all()
+
+
+@pytest.mark.parametrize("form", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+@pytest.mark.parametrize("rows,units,inner", [(1, 5, 70), (40, 300, 128), (161, 257, 1000), (257, 513, 1300), (700, 1111, 2500), (2600, 2100, 640)])
+def test_scaled_matmul_every_form(head, knobs, rows, units, inner, scale_dtype, form):
+    """Every tile form and the split-K form, whole and cut along K, ragged at all edges."""
+    knobs.setenv("FRCNN_PRODUCT_FORM", form)
+    a, sa, b, sb = operands(rows, units, inner, scale_dtype, form)
+    bias = torch.randn((units,), generator=gen(5), device="cuda")
+    want, size = product64(a, sa, b, sb, bias, None)
+    for out_dtype in (F32, F16, BF16):
+        y = head.scaled_matmul(a, sa, b, sb, bias=bias, out_dtype=out_dtype)
+        worst = ((y.double() - want).abs() - product_tolerance(want, size, inner, out_dtype)).max().item()
+        assert worst <= 0, (out_dtype, worst)
 
 
 def test_scaled_matmul_empty(head):
@@ -316,6 +333,24 @@ def test_group_norm(head, shape, groups, dtype, activation):
     check_norm(dbeta, r["dbeta"], r["off_dbeta"], F32, "dbeta")
     again = head.group_norm_gradients(dy, x, gamma, beta, stats, activation=activation)
     assert torch.equal(dx, again[0]) and torch.equal(dgamma, again[1]) and torch.equal(dbeta, again[2])
+
+
+@pytest.mark.parametrize("activation", [None, "swish"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,groups", [((1, 1, 8), 1), ((2, 5, 24), 3), ((3, 7, 7, 64), 32), ((2, 31, 31, 46), 2), ((1, 700, 1024), 1)])
+def test_group_norm_by_chunks(head, knobs, shape, groups, dtype, activation):
+    """The two-pass form at sizes that one workgroup would hold."""
+    knobs.setenv("FRCNN_NORM_CHUNKED", 1)
+    c = shape[-1]
+    x, dy = (torch.randn(shape, generator=gen(i), device="cuda").to(dtype) for i in (1, 2))
+    gamma, beta = 1 + 0.3 * torch.randn(c, generator=gen(3), device="cuda"), torch.randn(c, generator=gen(4), device="cuda")
+    r = norm64(x, gamma, beta, groups, 1e-3, activation, dy)
+    y, stats = head.group_norm(x, gamma, beta, groups, activation=activation, return_stats=True)
+    check_norm(y, r["y"], r["off_y"], dtype, "y")
+    check_norm(stats, r["stats"], r["off_stats"], F32, "stats")
+    assert torch.equal(y, head.group_norm(x, gamma, beta, groups, activation=activation))
+    for got, name in zip(head.group_norm_gradients(dy, x, gamma, beta, stats, activation=activation), ("dx", "dgamma", "dbeta")):
+        check_norm(got, r[name], r["off_" + name], dtype if name == "dx" else F32, name)
 
 
 @pytest.mark.parametrize("shape,groups", [((3, 7, 7, 64), 8), ((1, 9000, 64), 4)])
@@ -470,6 +505,38 @@ def test_dropout_gradient(head):
     one = torch.zeros_like(x)
     one[100, 3] = 1.0
     assert torch.equal(head.dropout(one, 0.25, 4, 9)[100, 3], dropped(torch.ones((333, 7), device="cuda"), 0.25, 4, 9)[100, 3])
+
+
+# ---- tensors of more than 2^32 elements ---------------------------------------------------------------------------------------------
+def test_offsets_beyond_32_bits(head):
+    rows, inner = 155000, 28224
+    assert rows * inner > 2 ** 32
+    x = torch.empty((rows, inner), dtype=BF16, device="cuda").fill_(0.5)
+    pick = torch.tensor([0, 1, 76084, 76085, rows - 2, rows - 1], device="cuda")
+    x[pick] = torch.randn((6, inner), generator=gen(1), device="cuda").bfloat16()
+    q, s = head.quantize_blocks(x)
+    want_q, want_s = quantized(x[pick], 1, F32)
+    picked = q.view(torch.uint8)[pick].view(torch.float8_e4m3fn)
+    assert torch.equal(picked.float().double(), want_q) and torch.equal(s[pick].double(), want_s)
+    b, sb = head.quantize_blocks(torch.randn((40, inner), generator=gen(2), device="cuda"), block_rows=128)
+    y = head.scaled_matmul(q, s, b, sb)
+    want, size = product64(picked, s[pick], b, sb, None, None)
+    assert ((y[pick].double() - want).abs() - product_tolerance(want, size, inner, BF16)).max().item() <= 0
+    del q, s, y
+    z = head.dropout(x, 0.25, 7, 3)
+    for r in (76085, rows - 1):
+        words = philox(np.arange(r * inner // 4, (r + 1) * inner // 4), 7, 3).reshape(-1)
+        keep = torch.from_numpy(words >= np.uint64(2 ** 30)).cuda()
+        assert torch.equal(z[r], torch.where(keep, x[r].float() * float(np.float32(4 / 3)), 0.0).to(BF16))
+    del z
+    gamma, beta = torch.ones(576, device="cuda"), torch.zeros(576, device="cuda")
+    maps = x.view(rows, 49, 576)
+    y, stats = head.group_norm(maps, gamma, beta, 32, return_stats=True)
+    r = norm64(maps[pick], gamma, beta, 32, 1e-3, None, maps[pick])
+    check_norm(y[pick], r["y"], r["off_y"], BF16, "y")
+    dx, dgamma, dbeta = head.group_norm_gradients(maps, maps, gamma, beta, stats)
+    check_norm(dx[pick], r["dx"], r["off_dx"], BF16, "dx")
+    assert torch.isfinite(dgamma).all() and torch.isfinite(dbeta).all()
 
 
 # ---- streams, graphs ------------------------------------------------------------------------------------------------------------------
@@ -638,6 +705,11 @@ def test_training_head_steps():
         mask = dropped(torch.ones(x.shape, device="cuda"), 0.4, 77, i) != 0
         assert torch.equal(out[0] != 0, mask & (norm(x).detach() != 0))
     assert drop(x) is x
+    host = [drop(torch.ones(4000), training=True) for _ in range(2)]  # tensors of the host take part, with a new mask each
+    assert host[0].is_cuda and not torch.equal(host[0], host[1])
+    half = norm.gamma.detach().half().requires_grad_()  # parameters of another type get their gradient in it
+    pkg.head_utils.group_norm(x, half, norm.beta, 8).sum().backward()
+    assert half.grad.dtype == F16
     fresh = pkg.box_head.Dropout(0.4)
     with pytest.raises(RuntimeError, match="before capturing"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):

@@ -48,6 +48,8 @@ enum Knob {
   kKnobSortRadixOnly,    // FRCNN_SORT_RADIX_ONLY       1: sort_select_kernel orders its slots by the stable radix sort only
   kKnobBitmaskThreads,   // FRCNN_BITMASK_THREADS       256|1024: workgroup size of the whole-chip bitmask schedule's scan kernels
   kKnobCropStage,        // FRCNN_CROP_STAGE            0|1: frcnn_roi_pooling's LDS-staged-rows schedule (default: beyond 4 MiB per image)
+  kKnobProductForm,      // FRCNN_PRODUCT_FORM          0..3: frcnn_scaled_matmul's tile forms, 4: the split-K form (0 and 1: not for fp32 results)
+  kKnobNormChunked,      // FRCNN_NORM_CHUNKED          1: frcnn_group_norm and its gradients by chunks of positions
   kKnobCount
 };
 bool knob_set(Knob k);

@@ -694,7 +694,7 @@ static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, bo
   };
   for (const auto &c : choices) {
     most = c[0], limit = c[1];
-    p.resident = narrow_enough();
+    p.resident = !knob(kKnobNormChunked, 0) && narrow_enough();
     if (p.resident) break;
   }
   if (p.resident) {
@@ -849,7 +849,7 @@ static int norm_check(const char *what, int type, int64_t N, int64_t S, int C, i
   FRCNN_REQUIRE(N >= 0 && S >= 1, "%s: needs at least one position per image (N=%lld, S=%lld)", what, (long long)N, (long long)S);
   FRCNN_REQUIRE(C >= 1 && G >= 1 && C % G == 0, "%s: %d channels are not a multiple of %d groups", what, C, G);
   FRCNN_REQUIRE(act == FRCNN_ACT_NONE || act == FRCNN_ACT_RELU || act == FRCNN_ACT_SWISH, "%s: unknown activation %d", what, act);
-  if (N >= (1ll << 31) || S >= (1ll << 24) || C > (1 << 20) || N * G >= (1ll << 31) || N * C >= (1ll << 38))
+  if (N > (1ll << 30) || S >= (1ll << 24) || C > (1 << 20) || N * G >= (1ll << 31) || N * C >= (1ll << 38))
     return set_error(FRCNN_EUNSUPPORTED, "%s: (%lld, %lld, %d) is beyond what the kernels index", what, (long long)N, (long long)S, C);
   return FRCNN_OK;
 }

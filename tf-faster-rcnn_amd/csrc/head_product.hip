@@ -440,6 +440,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
     load_a.start(k0, smem);
     load_b.start(k0, bs);
     fetch_scales(k0);
+    __builtin_amdgcn_sched_barrier(0);  // the first barrier counts on this order
     if (DB == 3) load_b.start(min(k0 + 1, last - 1), bs + B);
     load_a.start(min(k0 + 1, last - 1), smem + A);
     int at = 0, bt = 0;  // offsets of this step's tiles
@@ -517,6 +518,10 @@ struct TileForm {
 static const TileForm kTileForms[] = {{256, 256, 1, 1.63f, 0.0f}, {160, 256, 1, 1.06f, 0.0f}, {128, 128, 2, 1.04f, 1.96f}, {64, 128, 2, 0.80f, 1.17f}};
 static const int kTileFormCount = sizeof(kTileForms) / sizeof(kTileForms[0]);
 
+static bool product_size_known(int M, int N, int K) {
+  return M <= (1 << 30) && N <= (1 << 24) && K <= (1 << 22) && (long long)((M + 63) / 64) * ((N + 63) / 64) < (1ll << 30);
+}
+
 static TilePlan tile_plan(const TileForm &f, int M, int N, int blocks) {
   TilePlan t;
   t.tiles_m = (M + f.bm - 1) / f.bm;
@@ -545,6 +550,8 @@ static double plan_us(const TileForm &f, const TilePlan &t, int blocks, bool wid
 }
 
 static int best_form(int M, int N, int blocks, bool wide) {
+  const int forced = knob(kKnobProductForm, -1);
+  if (forced >= 0 && forced < kTileFormCount && !(wide && kTileForms[forced].wide_us == 0.0f)) return forced;
   int best = 2;  // every result type has it
   double least = 1e30;
   for (int i = 0; i < kTileFormCount; ++i) {
@@ -557,7 +564,10 @@ static int best_form(int M, int N, int blocks, bool wide) {
 
 // A workgroup of product_split_kernel streams 4 KB per 16 x 16 tile and block through the chip at about 7.5 TB/s.
 static bool use_tiles(int M, int N, int blocks, bool wide) {
-  if (M <= 16 || blocks == 0) return false;
+  if (blocks == 0) return false;
+  const int forced = knob(kKnobProductForm, -1);
+  if (forced >= 0) return forced < kTileFormCount;
+  if (M <= 16) return false;
   const TileForm &f = kTileForms[best_form(M, N, blocks, wide)];
   const double split_us = 4.0 + (double)((M + 15) / 16) * ((N + 15) / 16) * blocks * 5.5e-4;
   return plan_us(f, tile_plan(f, M, N, blocks), blocks, wide) < split_us;
@@ -618,7 +628,7 @@ using namespace frcnn;
 extern "C" {
 
 size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K) {
-  if (M < 1 || N < 1 || K < 1) return 0;
+  if (M < 1 || N < 1 || K < 1 || !product_size_known(M, N, K)) return 0;
   const int blocks = (K + kQuantBlock - 1) / kQuantBlock;
   size_t most = 0;
   for (int wide = 0; wide < 2; ++wide) {  // the output's type decides
@@ -649,9 +659,9 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
     FRCNN_REQUIRE(a_scale_row_stride >= 0 && a_scale_block_stride >= 0 && b_scale_row_stride >= 0 && b_scale_block_stride >= 0,
                   "scaled_matmul: negative scale stride");
   }
-  if ((long long)((M + 63) / 64) * ((N + 63) / 64) >= (1ll << 30) || K > (1 << 22) || lda > (1 << 23) || ldb > (1 << 23) || N > (1 << 24))
-    return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: K=%d (row strides %lld, %lld), N=%d is beyond what the kernels index", K,
-                     (long long)lda, (long long)ldb, N);
+  if (!product_size_known(M, N, K) || lda > (1 << 23) || ldb > (1 << 23))
+    return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: M=%d, N=%d, K=%d (row strides %lld, %lld) is beyond what the kernels index", M, N, K,
+                     (long long)lda, (long long)ldb);
   const size_t need = frcnn_scaled_matmul_workspace_bytes(M, N, K);
   FRCNN_REQUIRE(need == 0 || (workspace && aligned_to(workspace, 256) && workspace_bytes >= need),
                 "scaled_matmul: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);

@@ -135,7 +135,7 @@ static int launch_quantize(const void *x, long long ldx, int rows, int K, void *
                            long long scale_row, long long scale_block, int power_of_two, hipStream_t stream) {
   const int across = (K + kQuantBlock - 1) / kQuantBlock;
   const int per = BR == 1 ? 64 : 128;
-  const long long blocks = (long long)((rows + per - 1) / per) * across;
+  const long long blocks = ((long long)rows + per - 1) / per * across;
   if (blocks >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "quantize_blocks: too many blocks");
   const bool vector = aligned_to(x, 16) && (ldx * (long long)sizeof(T)) % 16 == 0;
   if (vector)

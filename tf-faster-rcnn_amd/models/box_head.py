@@ -117,7 +117,7 @@ class Dropout(Layer):
         if not 0.0 <= self.rate < 1.0:
             raise ValueError(f"rate must be in [0, 1), got {rate}")
         self.seed = seed
-        self._state: Optional[torch.Tensor] = None
+        self._states: Dict[torch.device, torch.Tensor] = {}
 
     def get_config(self) -> Dict[str, Any]:
         config = super().get_config()
@@ -128,13 +128,14 @@ class Dropout(Layer):
         """Any shape, fp32, fp16 or bf16; the input itself when not training or at rate 0."""
         if not training or self.rate == 0.0:
             return inputs
-        if self._state is None or self._state.device != inputs.device:
+        inputs = head_utils._operand(inputs, "inputs")
+        state = self._states.get(inputs.device)
+        if state is None:
             if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"{self.name}: call the layer once before capturing it")
             seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if self.seed is None else int(self.seed)
             seed = (seed + 2 ** 63) % 2 ** 64 - 2 ** 63  # the 64 bits as a signed integer
-            device = inputs.device if inputs.is_cuda else _lib.require_gpu()
-            self._state = torch.tensor([seed, 0], dtype=torch.int64, device=device)
-        used = self._state.clone()
-        self._state[1:].add_(1)
+            state = self._states[inputs.device] = torch.tensor([seed, 0], dtype=torch.int64, device=inputs.device)
+        used = state.clone()
+        state[1:].add_(1)
         return head_utils.dropout(inputs, self.rate, used)

@@ -48,7 +48,7 @@ def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
                 raise ValueError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
-def _leaves_of(*tensors: torch.Tensor) -> None:
+def _leaves_of(*tensors: Any) -> None:
     """Refuse a capture that the backward pass would end the process in.
 
     autograd runs a leaf's accumulation node on the stream on which the node was made, and the node lives as long as any
@@ -56,7 +56,7 @@ def _leaves_of(*tensors: torch.Tensor) -> None:
     stream, which the runtime does not survive.  The node keeps a note of the stream on which it was first met here.
     """
     for t in tensors:
-        if t.requires_grad and t.is_leaf:
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.requires_grad and t.is_leaf:
             stream = _lib.stream_ptr(t.device)
             made_on = torch.autograd.graph.get_gradient_edge(t).node.metadata.setdefault("frcnn_stream", stream)
             if made_on != stream and torch.cuda.is_current_stream_capturing():
@@ -266,6 +266,7 @@ def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     Returns:
         ``y`` of ``x``'s shape and type, or ``(y, stats)``.  Differentiable by ``x``, ``gamma`` and ``beta`` (once).
     """
+    given = (x, gamma, beta)
     x = _operand(x, "x").contiguous()
     act = _activation(activation, (None, "linear", "relu", "swish"))
     _, _, channels = _norm_shape(x, groups)
@@ -274,7 +275,7 @@ def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     if not epsilon >= 0.0:
         raise ValueError(f"epsilon must not be negative, got {epsilon}")
     if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
-        _leaves_of(x, gamma, beta)
+        _leaves_of(*given)
         y, stats = _GroupNorm.apply(x, gamma, beta, int(groups), epsilon, act)
     else:
         y, stats = _norm_forward(x, gamma, beta, int(groups), epsilon, act, return_stats)
@@ -341,7 +342,7 @@ def dropout(x: torch.Tensor, rate: float, seed: Any, offset: int = 0) -> torch.T
             captured graph that advances it draws a new mask at each replay.
         offset: 64-bit integer, a stream of its own under the same seed (one per call and layer).
     """
-    x = _operand(x, "x").contiguous()
+    given, x = x, _operand(x, "x").contiguous()
     rate = float(rate)
     if not 0.0 <= rate < 1.0:
         raise ValueError(f"rate must be in [0, 1), got {rate}")
@@ -354,6 +355,6 @@ def dropout(x: torch.Tensor, rate: float, seed: Any, offset: int = 0) -> torch.T
         state, seed = seed.contiguous(), 0
     seed, offset = int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF
     if torch.is_grad_enabled() and x.requires_grad:
-        _leaves_of(x)
+        _leaves_of(given)
         return _Dropout.apply(x, rate, seed, offset, state)
     return _dropout(x, rate, seed, offset, state)
