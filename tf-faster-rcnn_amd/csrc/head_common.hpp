@@ -68,7 +68,14 @@ struct Pack {
     }
     return o;
   }
-  __device__ __forceinline__ static void store(T *p, const float (&f)[VEC]) { *reinterpret_cast<u32x4 *>(p) = packed(f); }
+  // PAST: past the caches, for results that fill whole lines
+  template <bool PAST = false>
+  __device__ __forceinline__ static void store(T *p, const float (&f)[VEC]) {
+    if constexpr (PAST)
+      __builtin_nontemporal_store(packed(f), reinterpret_cast<u32x4 *>(p));
+    else
+      *reinterpret_cast<u32x4 *>(p) = packed(f);
+  }
 };
 
 template <typename T>
@@ -77,6 +84,7 @@ struct Pack<T, 1> {
   __device__ __forceinline__ static Pack load(const T *p) { return Pack{*p}; }
   __device__ __forceinline__ static Pack zero() { return Pack{(T)0.0f}; }
   __device__ __forceinline__ void unpack(float (&f)[1]) const { f[0] = to_float(w); }
+  template <bool PAST = false>
   __device__ __forceinline__ static void store(T *p, const float (&f)[1]) { *p = (T)f[0]; }
 };
 
