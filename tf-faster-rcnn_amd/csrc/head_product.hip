@@ -129,16 +129,25 @@ __device__ __forceinline__ void multiply(const typename Operand<MODE>::type &w, 
     add_scaled(acc, block_product<MODE>(w, a, f32x4{0, 0, 0, 0}, sw, sa), sw * sa);
 }
 
-// Bias, activation, rounding and store of four neighbouring columns n .. n + 3 of row m.
+// The bias of columns n .. n + 3; zeros without one or beyond the last column.
+__device__ __forceinline__ f32x4 bias4(const ProductArgs &p, int n) {
+  f32x4 v = {0, 0, 0, 0};
+  if (!p.bias || n >= p.N) return v;
+  if (p.quads) return *reinterpret_cast<const f32x4 *>(p.bias + n);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < p.N) v[i] = p.bias[n + i];
+  return v;
+}
+
+// Activation, rounding and store of four neighbouring columns n .. n + 3 of row m.
 template <typename T>
 __device__ __forceinline__ void store4(const ProductArgs &p, int m, int n, f32x4 v) {
-  if (m >= p.M || n >= p.N) return;
   T *row = reinterpret_cast<T *>(p.y) + (long long)m * p.ldy + n;
-  if (p.quads) {
-    if (p.bias) v += *reinterpret_cast<const f32x4 *>(p.bias + n);
-    if (p.act == FRCNN_ACT_RELU)
+  if (p.act == FRCNN_ACT_RELU)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = v[i] > 0.0f ? v[i] : (v[i] != v[i] ? v[i] : 0.0f);
+    for (int i = 0; i < 4; ++i) v[i] = v[i] > 0.0f ? v[i] : (v[i] != v[i] ? v[i] : 0.0f);
+  if (p.quads) {
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<f32x4 *>(row) = v;
     } else {
@@ -149,11 +158,7 @@ __device__ __forceinline__ void store4(const ProductArgs &p, int m, int n, f32x4
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (n + i < p.N) {
-      float f = v[i] + (p.bias ? p.bias[n + i] : 0.0f);
-      if (p.act == FRCNN_ACT_RELU) f = f > 0.0f ? f : (f != f ? f : 0.0f);
-      row[i] = (T)f;
-    }
+    if (n + i < p.N) row[i] = (T)v[i];
 }
 
 // f(T) for the output's type T: one uniform branch around all of a thread's stores.
@@ -221,9 +226,9 @@ __global__ __launch_bounds__(64 * W) void product_split_kernel(ProductArgs p, in
     f32x4 v = part[0][t][lane];
 #pragma unroll
     for (int w = 1; w < W; ++w) v += part[w][t][lane];
-    with_output_type(p, [&](auto *type) {
-      store4<__remove_pointer(decltype(type))>(p, m0 + (t / TN) * 16 + (lane & 15), n0 + (t % TN) * 16 + (lane >> 4) * 4, v);
-    });
+    const int m = m0 + (t / TN) * 16 + (lane & 15), n = n0 + (t % TN) * 16 + (lane >> 4) * 4;
+    v += bias4(p, n);
+    if (m < p.M && n < p.N) with_output_type(p, [&](auto *type) { store4<__remove_pointer(decltype(type))>(p, m, n, v); });
   }
 }
 
@@ -480,12 +485,20 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
 #pragma unroll
       for (int j = 0; j < NT; ++j) out[(i * NT + j) * THREADS] = acc[i][j];
   } else {
+    f32x4 bias[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) bias[j] = bias4(p, n0 + wn + j * 16 + (lane >> 4) * 4);
     with_output_type(p, [&](auto *type) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i) {
+        const int m = m0 + wm + i * 16 + (lane & 15);
+        if (m < p.M)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          store4<__remove_pointer(decltype(type))>(p, m0 + wm + i * 16 + (lane & 15), n0 + wn + j * 16 + (lane >> 4) * 4, acc[i][j]);
+          for (int j = 0; j < NT; ++j) {
+            const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+            if (n < p.N) store4<__remove_pointer(decltype(type))>(p, m, n, acc[i][j] + bias[j]);
+          }
+      }
     });
   }
 }
@@ -504,7 +517,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_join_kernel(ProductArgs 
   f32x4 v = in[0];
 #pragma unroll 8
   for (int i = 1; i < plan.pieces; ++i) v += in[(long long)i * (MT * NT * THREADS)];
-  with_output_type(p, [&](auto *type) { store4<__remove_pointer(decltype(type))>(p, m, n, v); });
+  v += bias4(p, n);
+  if (m < p.M && n < p.N) with_output_type(p, [&](auto *type) { store4<__remove_pointer(decltype(type))>(p, m, n, v); });
 }
 
 // The tile forms, and how long one takes for a block of 128 columns when the chip is full of them (measured between K = 8320 and

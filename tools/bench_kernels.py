@@ -167,6 +167,54 @@ def case_decoder(name, B, R, L, iters):
                 images_per_s=B / (ms * 1e-3))
 
 
+def rotate(make, call):
+    """`call` on three sets of inputs in turn, which together exceed the caches at the head's larger sizes."""
+    sets, turn = [make(i) for i in range(3)], [0]
+
+    def nxt():
+        turn[0] += 1
+        return call(*sets[turn[0] % 3])
+    return nxt
+
+
+def case_product(name, rows, units, inner, scales, out, iters):
+    """A dense layer of the detection head in e4m3 with block scales; flops beside the bytes, since the large ones are not HBM bound."""
+    hu = pkg.head_utils
+
+    def make(i):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        x = torch.randn((rows, inner), generator=g, device="cuda").clamp_min_(0)
+        w = torch.randn((units, inner), generator=g, device="cuda").mul_(inner ** -0.5)
+        return (*hu.quantize_blocks(x, scale_dtype=scales), *hu.quantize_blocks(w, 128, scale_dtype=scales))
+    bias = torch.zeros(units, device="cuda")
+    ms = timeit(rotate(make, lambda a, sa, b, sb: hu.scaled_matmul(a, sa, b, sb, bias=bias, activation="relu", out_dtype=out)), iters)
+    return {"case": name, "ms": ms, "bytes": rows * inner + units * inner + rows * units * torch.finfo(out).bits // 8,
+            "TFLOPs": round(2 * rows * units * inner / ms / 1e9, 1)}
+
+
+def case_quantize(name, rows, inner, dtype, iters):
+    ms = timeit(rotate(lambda i: (torch.randn((rows, inner), device="cuda").to(dtype),), pkg.head_utils.quantize_blocks), iters)
+    return {"case": name, "ms": ms, "bytes": rows * inner * (torch.finfo(dtype).bits // 8 + 1)}
+
+
+def case_norm(name, shape, dtype, activation, grad, iters):
+    hu, c = pkg.head_utils, shape[-1]
+    gamma, beta = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+
+    def call(x, dy):
+        y, stats = hu.group_norm(x, gamma, beta, 32, activation=activation, return_stats=True)
+        return hu.group_norm_gradients(dy, x, gamma, beta, stats, activation=activation) if grad else y
+    ms = timeit(rotate(lambda i: tuple(torch.randn(shape, device="cuda").to(dtype) for _ in range(2)), call), iters)
+    return {"case": name, "ms": ms, "bytes": (5 if grad else 2) * int(np.prod(shape)) * torch.finfo(dtype).bits // 8}
+
+
+def case_dropout(name, shape, dtype, iters):
+    ms = timeit(rotate(lambda i: (torch.randn(shape, device="cuda").to(dtype),), lambda x: pkg.head_utils.dropout(x, 0.5, 1)), iters)
+    return {"case": name, "ms": ms, "bytes": 2 * int(np.prod(shape)) * torch.finfo(dtype).bits // 8}
+
+
+F32, F16, BF16, E8M0 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e8m0fnu
+
 CASES = {
     "crop_cfg1": lambda it: case_crop("crop_cfg1", 1, 32, 576, 300, 6000, it),  # one image: the small-launch four-slice schedule
     "crop_cfg2": lambda it: case_crop("crop_cfg2", 16, 32, 576, 300, 6000, it),
@@ -184,6 +232,17 @@ CASES = {
     "roi_bbox_cfg3": lambda it: case_roi_bbox("roi_bbox_cfg3", 16, 31, 6000, 2000, it, mode="training"),
     "roi_bbox_cfg5": lambda it: case_roi_bbox("roi_bbox_cfg5", 16, 63, 12000, 300, it),
     "decoder_cfg2": lambda it: case_decoder("decoder_cfg2", 16, 300, 21, it),
+    # the detection head between RoIPooling and Decoder
+    "head_fc1_row": lambda it: case_product("head_fc1_row", 1, 4096, 28224, F32, BF16, it),
+    "head_fc1_image": lambda it: case_product("head_fc1_image", 300, 4096, 28224, F32, BF16, it),
+    "head_fc1_batch": lambda it: case_product("head_fc1_batch", 4800, 4096, 28224, F32, BF16, it),
+    "head_fc2_batch": lambda it: case_product("head_fc2_batch", 4800, 4096, 4096, E8M0, BF16, it),
+    "head_scores": lambda it: case_product("head_scores", 300, 105, 4096, F32, F32, it),
+    "head_quantize": lambda it: case_quantize("head_quantize", 4800, 28224, F32, it),
+    "head_norm_maps": lambda it: case_norm("head_norm_maps", (16, 32, 32, 576), F32, "relu", False, it),
+    "head_norm_pooled_train": lambda it: case_norm("head_norm_pooled_train", (6000, 7, 7, 512), BF16, "swish", True, it),
+    "head_norm_maps_train": lambda it: case_norm("head_norm_maps_train", (8, 63, 63, 512), F16, "swish", True, it),
+    "head_dropout": lambda it: case_dropout("head_dropout", (6000, 4096), F32, it),
 }
 
 
