@@ -26,6 +26,7 @@ struct ProductArgs {
   int M, N, K, blocks;  // blocks = ceil(K / 128)
   int act, out;
   int quads;  // N, ldy and the pointers allow four columns at a time
+  int rows16;  // y's rows start at multiples of 16 bytes
 };
 
 // The 16 bytes at `col` of a row of K bytes; bytes at K and beyond are zero.
@@ -129,6 +130,8 @@ __device__ __forceinline__ void multiply(const typename Operand<MODE>::type &w, 
     add_scaled(acc, block_product<MODE>(w, a, f32x4{0, 0, 0, 0}, sw, sa), sw * sa);
 }
 
+__device__ __forceinline__ float relu(float v) { return v > 0.0f ? v : (v != v ? v : 0.0f); }
+
 // The bias of columns n .. n + 3; zeros without one or beyond the last column.
 __device__ __forceinline__ f32x4 bias4(const ProductArgs &p, int n) {
   f32x4 v = {0, 0, 0, 0};
@@ -146,7 +149,7 @@ __device__ __forceinline__ void store4(const ProductArgs &p, int m, int n, f32x4
   T *row = reinterpret_cast<T *>(p.y) + (long long)m * p.ldy + n;
   if (p.act == FRCNN_ACT_RELU)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = v[i] > 0.0f ? v[i] : (v[i] != v[i] ? v[i] : 0.0f);
+    for (int i = 0; i < 4; ++i) v[i] = relu(v[i]);
   if (p.quads) {
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<f32x4 *>(row) = v;
@@ -160,6 +163,30 @@ __device__ __forceinline__ void store4(const ProductArgs &p, int m, int n, f32x4
   for (int i = 0; i < 4; ++i)
     if (n + i < p.N) row[i] = (T)v[i];
 }
+
+// 16 rows from m and 16 NT columns from n, all of them columns of y, by way of the wave's own piece of LDS: a store instruction
+// then fills whole rows of the tile instead of 32 bytes of each.
+template <typename T, int NT>
+struct RowStore {
+  static constexpr int ROW = NT * 16 * sizeof(T), STRIDE = ROW + 16, BYTES = 16 * STRIDE;
+  static constexpr int LANES = ROW / 16, PER = 64 / LANES;  // lanes per row, rows per store
+  __device__ __forceinline__ static void run(const ProductArgs &p, uint8_t *scratch, int m, int n, f32x4 (&v)[NT]) {
+    typedef T tx4 __attribute__((ext_vector_type(4)));
+    const int lane = lane_id();
+    uint8_t *to = scratch + (lane & 15) * STRIDE + (lane >> 4) * 4 * sizeof(T);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *reinterpret_cast<tx4 *>(to + j * 16 * sizeof(T)) = __builtin_convertvector(v[j], tx4);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's lanes read what others of them wrote
+    const int row = lane / LANES, chunk = lane % LANES;
+    T *out = reinterpret_cast<T *>(p.y) + (long long)(m + row) * p.ldy + n + chunk * (16 / sizeof(T));
+#pragma unroll
+    for (int s = 0; s < 16 / PER; ++s) {
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(scratch + (s * PER + row) * STRIDE + chunk * 16);
+      if (m + s * PER + row < p.M) *reinterpret_cast<u32x4 *>(out + (long long)s * PER * p.ldy) = w;
+    }
+    asm volatile("" ::: "memory");
+  }
+};
 
 // f(T) for the output's type T: one uniform branch around all of a thread's stores.
 template <typename F>
@@ -477,6 +504,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
     take_scales();
     step_barrier<0>();
     compute(smem, bs, [](int) {});
+    step_barrier<0>();  // LDS is free for the results
   }
   if (piece >= 0) {
     f32x4 *out = partial + (long long)piece * (MT * NT * THREADS) + threadIdx.x;
@@ -488,7 +516,26 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
     f32x4 bias[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) bias[j] = bias4(p, n0 + wn + j * 16 + (lane >> 4) * 4);
+    const bool whole_rows = p.rows16 && n0 + wn + NT * 16 <= p.N;
     with_output_type(p, [&](auto *type) {
+      using T = __remove_pointer(decltype(type));
+      using R = RowStore<T, NT>;
+      static_assert(R::BYTES * WM * WN <= 3 * A + DB * B, "the waves' pieces of LDS");
+      if (whole_rows) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          f32x4 v[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            v[j] = acc[i][j] + bias[j];
+            if (p.act == FRCNN_ACT_RELU)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[j][e] = relu(v[j][e]);
+          }
+          R::run(p, smem + wave * R::BYTES, m0 + wm + i * 16, n0 + wn, v);
+        }
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int m = m0 + wm + i * 16 + (lane & 15);
@@ -496,7 +543,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-            if (n < p.N) store4<__remove_pointer(decltype(type))>(p, m, n, acc[i][j] + bias[j]);
+            if (n < p.N) store4<T>(p, m, n, acc[i][j] + bias[j]);
           }
       }
     });
@@ -680,9 +727,10 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
   FRCNN_REQUIRE(need == 0 || (workspace && aligned_to(workspace, 256) && workspace_bytes >= need),
                 "scaled_matmul: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);
   const int quads = N % 4 == 0 && ldy % 4 == 0 && aligned_to(y, 4 * type_bytes(y_type)) && aligned_to(bias, 16);
+  const int rows16 = (ldy * (int64_t)type_bytes(y_type)) % 16 == 0 && aligned_to(y, 16);
   const ProductArgs p = {(const uint8_t *)a, (const uint8_t *)b, lda, ldb, a_scales, b_scales, a_scale_row_stride, a_scale_block_stride,
                          b_scale_row_stride, b_scale_block_stride, bias, y, ldy, M, N, K, (K + kQuantBlock - 1) / kQuantBlock,
-                         activation, y_type, quads};
+                         activation, y_type, quads, rows16};
   const int mode = (y_type == FRCNN_F32 ? kWideF32 : kNarrowF32) + (scale_type == FRCNN_SCALE_E8M0);
   hipStream_t s = (hipStream_t)stream;
   if (mode == kNarrowF32) return launch_product<kNarrowF32>(p, workspace, workspace_bytes, s);
