@@ -17,6 +17,8 @@ from .. import _lib
 
 BLOCK = 128
 
+_E4M3 = torch.float8_e4m3fn
+_E4M3_ONLY = (_E4M3,)
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _SCALE_TYPES = {torch.float32: 0, torch.float8_e8m0fnu: 1}
 _ACTIVATIONS = {None: 0, "linear": 0, "relu": 1, "swish": 2}
@@ -62,6 +64,18 @@ def _leaves_of(*tensors: Any) -> None:
             if made_on != stream and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("an eager autograd graph of the same leaf is alive, so the captured backward pass would wait for its "
                                    "stream: delete what that graph returned, or capture with leaves of its own")
+
+
+def _run(device: torch.device, function: Any, *args: Any) -> None:
+    """One call through the C ABI, on ``device`` and its current stream."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
@@ -113,12 +127,10 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1,
     across, up = -(-inner // BLOCK), -(-rows // block_rows)
     # rows of a block or more start at whole lines of memory: the product reads them a line at a time
     wide = -(-inner // BLOCK) * BLOCK if inner >= BLOCK else -(-inner // 16) * 16
-    q = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=device)
+    q = flat.new_empty((rows, wide), dtype=_E4M3)
     scales = torch.empty_strided((up, across), (1, up), dtype=scale_dtype, device=device)
-    with _lib.on_device(device):
-        _lib.check(_lib.lib().frcnn_quantize_blocks(flat.data_ptr(), _TYPES[x.dtype], max(stride, inner), rows, inner, block_rows,
-                                                    q.data_ptr(), wide, scales.data_ptr(), _SCALE_TYPES[scale_dtype], 1, up,
-                                                    _lib.stream_ptr(device)))
+    _run(device, _lib.lib().frcnn_quantize_blocks, flat.data_ptr(), _TYPES[x.dtype], max(stride, inner), rows, inner, block_rows,
+         q.data_ptr(), wide, scales.data_ptr(), _SCALE_TYPES[scale_dtype], 1, up)
     q = q[:, :inner] if wide != inner else q
     return (q if len(lead) == 1 else q.unflatten(0, lead) if lead else q[0]), scales
 
@@ -141,13 +153,13 @@ def scaled_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
         ``(..., N)`` of ``out_dtype``; sums are held in fp32.  Rows of ``a`` or ``b`` that do not start at multiples of 16
         bytes are copied first; ``quantize_blocks`` returns rows that do.  No gradient is defined.
     """
-    a = _operand(a, "a", (torch.float8_e4m3fn,))
+    a = _operand(a, "a", _E4M3_ONLY)
     device = a.device
-    b = _operand(b, "b", (torch.float8_e4m3fn,), device)
+    b = _operand(b, "b", _E4M3_ONLY, device)
     a_scales = _operand(a_scales, "a_scales", _SCALE_TYPES, device)
     b_scales = _operand(b_scales, "b_scales", _SCALE_TYPES, device)
     if bias is not None:
-        bias = _lib.device_tensor(bias, torch.float32, device)
+        bias = _parameter(bias, device)
     _no_gradient("scaled_matmul", a, b, a_scales, b_scales, bias)
     act = _activation(activation, (None, "linear", "relu"))
     if out_dtype not in _TYPES:
@@ -167,16 +179,15 @@ def scaled_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
     if bias is not None and bias.shape != (units,):
         raise ValueError(f"bias must be ({units},), got {tuple(bias.shape)}")
     a, b = _rows_of_16(a), _rows_of_16(b)
-    out = torch.empty((rows, units), dtype=out_dtype, device=device)
+    out = a.new_empty((rows, units), dtype=out_dtype)
     lib = _lib.lib()
     pad = -(-inner // 16) * 16
     nbytes = lib.frcnn_scaled_matmul_workspace_bytes(rows, units, inner)
     ws = _workspace(nbytes, device) if nbytes else None
-    with _lib.on_device(device):
-        _lib.check(lib.frcnn_scaled_matmul(a.data_ptr(), a.stride(0) if rows > 1 else pad, a_scales.data_ptr(), *a_scales.stride(),
-                                           b.data_ptr(), b.stride(0) if units > 1 else pad, b_scales.data_ptr(), *b_scales.stride(),
-                                           _SCALE_TYPES[a_scales.dtype], _lib.ptr(bias), act, rows, units, inner, out.data_ptr(),
-                                           _TYPES[out_dtype], units, _lib.ptr(ws), nbytes, _lib.stream_ptr(device)))
+    _run(device, lib.frcnn_scaled_matmul, a.data_ptr(), a.stride(0) if rows > 1 else pad, a_scales.data_ptr(), *a_scales.stride(),
+         b.data_ptr(), b.stride(0) if units > 1 else pad, b_scales.data_ptr(), *b_scales.stride(), _SCALE_TYPES[a_scales.dtype],
+         None if bias is None else bias.data_ptr(), act, rows, units, inner, out.data_ptr(), _TYPES[out_dtype], units,
+         None if ws is None else ws.data_ptr(), nbytes)
     return out if len(lead) == 1 else out.view(*lead, units)
 
 
@@ -191,52 +202,53 @@ def _norm_shape(x: torch.Tensor, groups: int) -> Tuple[int, int, int]:
     return batch, positions, channels
 
 
+def _parameter(p: Any, device: torch.device) -> torch.Tensor:
+    if p.__class__ is torch.Tensor and p.dtype is torch.float32 and p.device == device and p.is_contiguous():
+        return p
+    return _lib.device_tensor(p, torch.float32, device)
+
+
 def _parameters(gamma: Any, beta: Any, channels: int, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
-    gamma, beta = _lib.device_tensor(gamma, torch.float32, device), _lib.device_tensor(beta, torch.float32, device)
+    gamma, beta = _parameter(gamma, device), _parameter(beta, device)
     if gamma.shape != (channels,) or beta.shape != (channels,):
         raise ValueError(f"gamma and beta must be ({channels},), got {tuple(gamma.shape)} and {tuple(beta.shape)}")
     return gamma, beta
 
 
-def _norm_forward(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups: int, epsilon: float, act: int,
-                  want_stats: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    batch, positions, channels = _norm_shape(x, groups)
+def _norm_forward(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, shape: Tuple[int, int, int], groups: int, epsilon: float,
+                  act: int, want_stats: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    batch, positions, channels = shape
     device = x.device
     y = torch.empty_like(x)
     stats = torch.empty((batch, groups, 2), dtype=torch.float32, device=device) if want_stats else None
     lib = _lib.lib()
     nbytes = lib.frcnn_group_norm_workspace_bytes(_TYPES[x.dtype], batch, positions, channels, groups)
     ws = _workspace(nbytes, device) if nbytes else None
-    with _lib.on_device(device):
-        _lib.check(lib.frcnn_group_norm(_lib.ptr(x), _TYPES[x.dtype], batch, positions, channels, groups, _lib.ptr(gamma),
-                                        _lib.ptr(beta), epsilon, act, _lib.ptr(y), _lib.ptr(stats), _lib.ptr(ws), nbytes,
-                                        _lib.stream_ptr(device)))
+    _run(device, lib.frcnn_group_norm, x.data_ptr(), _TYPES[x.dtype], batch, positions, channels, groups, gamma.data_ptr(),
+         beta.data_ptr(), epsilon, act, y.data_ptr(), _lib.ptr(stats), _lib.ptr(ws), nbytes)
     return y, stats
 
 
 def _norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, stats: torch.Tensor,
-                   act: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    groups = stats.shape[1]
-    batch, positions, channels = _norm_shape(x, groups)
+                   shape: Tuple[int, int, int], act: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    (batch, positions, channels), groups = shape, stats.shape[1]
     device = x.device
     dx = torch.empty_like(x)
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
     lib = _lib.lib()
     nbytes = lib.frcnn_group_norm_grad_workspace_bytes(_TYPES[x.dtype], batch, positions, channels, groups)
     ws = _workspace(nbytes, device) if nbytes else None
-    with _lib.on_device(device):
-        _lib.check(lib.frcnn_group_norm_grad(_lib.ptr(dy), _lib.ptr(x), _TYPES[x.dtype], batch, positions, channels, groups,
-                                             _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(stats), act, _lib.ptr(dx), _lib.ptr(dgamma),
-                                             _lib.ptr(dbeta), _lib.ptr(ws), nbytes, _lib.stream_ptr(device)))
+    _run(device, lib.frcnn_group_norm_grad, dy.data_ptr(), x.data_ptr(), _TYPES[x.dtype], batch, positions, channels, groups,
+         gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), act, dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), _lib.ptr(ws), nbytes)
     return dx, dgamma, dbeta
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gamma, beta, groups, epsilon, act):  # type: ignore[override]
-        y, stats = _norm_forward(x, gamma, beta, groups, epsilon, act, True)
+    def forward(ctx, x, gamma, beta, shape, groups, epsilon, act):  # type: ignore[override]
+        y, stats = _norm_forward(x, gamma, beta, shape, groups, epsilon, act, True)
         ctx.save_for_backward(x, gamma, beta, stats)
-        ctx.act = act
+        ctx.act, ctx.shape = act, shape
         ctx.mark_non_differentiable(stats)
         return y, stats
 
@@ -244,8 +256,8 @@ class _GroupNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, _):  # type: ignore[override]
         x, gamma, beta, stats = ctx.saved_tensors
-        dx, dgamma, dbeta = _norm_backward(dy.contiguous(), x, gamma, beta, stats, ctx.act)
-        return dx, dgamma, dbeta, None, None, None
+        dx, dgamma, dbeta = _norm_backward(dy.contiguous(), x, gamma, beta, stats, ctx.shape, ctx.act)
+        return dx, dgamma, dbeta, None, None, None, None
 
 
 def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups: int, epsilon: float = 1e-3,
@@ -269,16 +281,16 @@ def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     given = (x, gamma, beta)
     x = _operand(x, "x").contiguous()
     act = _activation(activation, (None, "linear", "relu", "swish"))
-    _, _, channels = _norm_shape(x, groups)
-    gamma, beta = _parameters(gamma, beta, channels, x.device)
+    shape = _norm_shape(x, groups)
+    gamma, beta = _parameters(gamma, beta, shape[2], x.device)
     epsilon = float(epsilon)
     if not epsilon >= 0.0:
         raise ValueError(f"epsilon must not be negative, got {epsilon}")
     if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
         _leaves_of(*given)
-        y, stats = _GroupNorm.apply(x, gamma, beta, int(groups), epsilon, act)
+        y, stats = _GroupNorm.apply(x, gamma, beta, shape, int(groups), epsilon, act)
     else:
-        y, stats = _norm_forward(x, gamma, beta, int(groups), epsilon, act, return_stats)
+        y, stats = _norm_forward(x, gamma, beta, shape, int(groups), epsilon, act, return_stats)
     return (y, stats) if return_stats else y
 
 
@@ -292,23 +304,21 @@ def group_norm_gradients(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor,
     dy = _operand(dy, "dy", (x.dtype,), device).contiguous()
     if dy.shape != x.shape:
         raise ValueError(f"dy must be {tuple(x.shape)}, got {tuple(dy.shape)}")
-    stats = _lib.device_tensor(stats, torch.float32, device)
+    stats = _parameter(stats, device)
     if stats.dim() != 3 or stats.shape[0] != x.shape[0] or stats.shape[2] != 2:
         raise ValueError(f"stats must be ({x.shape[0]}, groups, 2), got {tuple(stats.shape)}")
     if stats.data_ptr() % 8:
         stats = stats.clone()
     act = _activation(activation, (None, "linear", "relu", "swish"))
-    _, _, channels = _norm_shape(x, stats.shape[1])
-    gamma, beta = _parameters(gamma, beta, channels, device)
+    shape = _norm_shape(x, stats.shape[1])
+    gamma, beta = _parameters(gamma, beta, shape[2], device)
     _no_gradient("group_norm_gradients", dy, x, gamma, beta, stats)
-    return _norm_backward(dy, x, gamma, beta, stats, act)
+    return _norm_backward(dy, x, gamma, beta, stats, shape, act)
 
 
 def _dropout(x: torch.Tensor, rate: float, seed: int, offset: int, state: Optional[torch.Tensor]) -> torch.Tensor:
     y = torch.empty_like(x)
-    with _lib.on_device(x.device):
-        _lib.check(_lib.lib().frcnn_dropout(_lib.ptr(x), _lib.ptr(y), _TYPES[x.dtype], x.numel(), rate, seed, offset, _lib.ptr(state),
-                                            _lib.stream_ptr(x.device)))
+    _run(x.device, _lib.lib().frcnn_dropout, x.data_ptr(), y.data_ptr(), _TYPES[x.dtype], x.numel(), rate, seed, offset, _lib.ptr(state))
     return y
 
 
