@@ -624,6 +624,34 @@ def test_captured_backward_beside_an_eager_graph(head):
         step()
 
 
+@pytest.mark.parametrize("eager", ["group_norm", "dropout", "strided dropout", "another operator"])
+def test_captured_call_beside_one_eager_graph(head, eager):
+    """One eager call is enough: each leaf of its graph is refused in a capture, and accepted once the graph is gone."""
+    x, other = (torch.randn((64, 3, 8), generator=gen(i), device="cuda", requires_grad=True) for i in (2, 3))
+    gamma, beta = (torch.ones(8, device="cuda", requires_grad=True) for _ in range(2))
+    strided = torch.randn((8, 3, 64), generator=gen(4), device="cuda").transpose(0, 2).requires_grad_()
+    graph_of = {"group_norm": lambda: head.group_norm(x, gamma, beta, 2), "dropout": lambda: head.dropout(x, 0.5, 1),
+                "strided dropout": lambda: head.dropout(strided, 0.5, 1), "another operator": lambda: x * 2}
+    refused = {"group_norm": [lambda: head.group_norm(x, beta.detach(), beta.detach(), 2), lambda: head.dropout(x, 0.5, 1),
+                              lambda: head.group_norm(other, gamma, beta.detach(), 2),
+                              lambda: head.group_norm(other, gamma.detach(), beta, 2)],
+               "dropout": [lambda: head.dropout(x, 0.5, 1), lambda: head.group_norm(x, gamma, beta, 2)],
+               "strided dropout": [lambda: head.dropout(strided, 0.5, 1)],
+               "another operator": [lambda: head.dropout(x, 0.5, 1)]}
+    alive = graph_of[eager]()
+    torch.cuda.synchronize()
+    for call in refused[eager]:
+        with pytest.raises(RuntimeError, match="alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    del alive
+    for call in refused[eager]:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call()  # and twice: the capture's own graph is alive
+            y = call()
+        del y
+
+
 def test_calls_on_two_streams(head):
     weights = weights_for(head, 49 * 64, 300, 64)
     state = torch.tensor([11, 0], device="cuda")

@@ -9,7 +9,7 @@ outputs and scratch from torch's allocator (so a captured graph owns them) and n
 
 from __future__ import annotations
 
-from typing import Any, Optional, Tuple
+from typing import Any, List, Optional, Tuple
 
 import torch
 
@@ -50,20 +50,34 @@ def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
                 raise ValueError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
-def _leaves_of(*tensors: Any) -> None:
+def _leaves_of(*tensors: Any) -> List[Any]:
     """Refuse a capture that the backward pass would end the process in.
 
     autograd runs a leaf's accumulation node on the stream on which the node was made, and the node lives as long as any
     graph of the leaf.  If an eager graph still holds it, a captured backward pass makes the capture wait for that other
-    stream, which the runtime does not survive.  The node keeps a note of the stream on which it was first met here.
+    stream, which the runtime does not survive.  The node keeps a note of the stream on which it was first met here; one that
+    others hold and that bears no note may be an eager graph's, and is refused in a capture too.
+
+    Returns the nodes: the caller keeps them until its own graph does, or the note would be gone with them.
     """
+    nodes = []
     for t in tensors:
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.requires_grad and t.is_leaf:
+        if isinstance(t, torch.Tensor) and t.requires_grad and t.is_leaf and t.is_cuda:
             stream = _lib.stream_ptr(t.device)
-            made_on = torch.autograd.graph.get_gradient_edge(t).node.metadata.setdefault("frcnn_stream", stream)
-            if made_on != stream and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("an eager autograd graph of the same leaf is alive, so the captured backward pass would wait for its "
-                                   "stream: delete what that graph returned, or capture with leaves of its own")
+            capturing = torch.cuda.is_current_stream_capturing()
+            node = torch.autograd.graph.get_gradient_edge(t).node
+            if capturing and "frcnn_stream" not in node.metadata:
+                node.metadata["frcnn_held"] = True
+                del node  # without another holder the node is gone now, and the next one is new
+                node = torch.autograd.graph.get_gradient_edge(t).node
+                if node.metadata.pop("frcnn_held", False):
+                    node.metadata["frcnn_stream"] = None
+            if node.metadata.setdefault("frcnn_stream", stream) != stream and capturing:
+                raise RuntimeError("an autograd graph of the same leaf, made before this capture or by another operator, is alive, so the "
+                                   "captured backward pass might wait for its stream: delete what that graph returned, or capture "
+                                   "with leaves of its own")
+            nodes.append(node)
+    return nodes
 
 
 def _run(device: torch.device, function: Any, *args: Any) -> None:
@@ -278,7 +292,7 @@ def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     Returns:
         ``y`` of ``x``'s shape and type, or ``(y, stats)``.  Differentiable by ``x``, ``gamma`` and ``beta`` (once).
     """
-    given = (x, gamma, beta)
+    held = _leaves_of(x, gamma, beta) if torch.is_grad_enabled() else None  # before anything here makes a node of them
     x = _operand(x, "x").contiguous()
     act = _activation(activation, (None, "linear", "relu", "swish"))
     shape = _norm_shape(x, groups)
@@ -287,10 +301,10 @@ def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     if not epsilon >= 0.0:
         raise ValueError(f"epsilon must not be negative, got {epsilon}")
     if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
-        _leaves_of(*given)
         y, stats = _GroupNorm.apply(x, gamma, beta, shape, int(groups), epsilon, act)
     else:
         y, stats = _norm_forward(x, gamma, beta, shape, int(groups), epsilon, act, return_stats)
+    del held  # the graph holds them
     return (y, stats) if return_stats else y
 
 
@@ -352,7 +366,8 @@ def dropout(x: torch.Tensor, rate: float, seed: Any, offset: int = 0) -> torch.T
             captured graph that advances it draws a new mask at each replay.
         offset: 64-bit integer, a stream of its own under the same seed (one per call and layer).
     """
-    given, x = x, _operand(x, "x").contiguous()
+    held = _leaves_of(x) if torch.is_grad_enabled() else None  # before anything here makes a node of it
+    x = _operand(x, "x").contiguous()
     rate = float(rate)
     if not 0.0 <= rate < 1.0:
         raise ValueError(f"rate must be in [0, 1), got {rate}")
@@ -365,6 +380,8 @@ def dropout(x: torch.Tensor, rate: float, seed: Any, offset: int = 0) -> torch.T
         state, seed = seed.contiguous(), 0
     seed, offset = int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF
     if torch.is_grad_enabled() and x.requires_grad:
-        _leaves_of(given)
-        return _Dropout.apply(x, rate, seed, offset, state)
-    return _dropout(x, rate, seed, offset, state)
+        y = _Dropout.apply(x, rate, seed, offset, state)
+    else:
+        y = _dropout(x, rate, seed, offset, state)
+    del held  # the graph holds it
+    return y
