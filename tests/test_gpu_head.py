@@ -652,6 +652,27 @@ def test_captured_call_beside_one_eager_graph(head, eager):
         del y
 
 
+def test_layers_make_their_state_outside_captures_and_modes(head):
+    from tf_faster_rcnn_amd.models.box_head import Dropout, GroupNormalization
+
+    x = torch.randn((4, 7, 7, 32), generator=gen(9), device="cuda")
+    for layer, args in ((GroupNormalization(8), {}), (Dropout(0.5, seed=1), {"training": True})):
+        with pytest.raises(RuntimeError, match="captur"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                layer(x, **args)
+        with torch.inference_mode():
+            layer(x, **args)
+        leaf = x.clone().requires_grad_()
+        y = layer(leaf, **args)
+        y.sum().backward()
+        assert leaf.grad.shape == x.shape
+    norm = GroupNormalization(8)
+    with torch.inference_mode():
+        norm.set_weights([torch.ones(32), torch.zeros(32)])
+    norm(x).sum().backward()
+    assert torch.allclose(norm.beta.grad, torch.full_like(norm.beta, 4 * 49))
+
+
 def test_calls_on_two_streams(head):
     weights = weights_for(head, 49 * 64, 300, 64)
     state = torch.tensor([11, 0], device="cuda")

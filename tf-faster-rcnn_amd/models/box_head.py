@@ -70,7 +70,7 @@ class GroupNormalization(Layer):
     """Group normalisation over the last axis' channels, with an activation.
 
     ``gamma`` and ``beta`` start as ones and zeros of the first input's channels; they are fp32 tensors that may require
-    gradients (``trainable``).
+    gradients (``trainable``).  A first call without ``set_weights`` makes them and may not itself be captured.
     """
 
     def __init__(self, groups: int = 32, epsilon: float = 1e-3, activation: Optional[str] = None, **kwargs: Any) -> None:
@@ -88,10 +88,11 @@ class GroupNormalization(Layer):
 
     def set_weights(self, weights: Sequence[torch.Tensor]) -> None:
         """``[gamma (channels,), beta (channels,)]``."""
-        gamma, beta = (_lib.device_tensor(w, torch.float32).detach().clone() for w in weights)
-        if gamma.dim() != 1 or gamma.shape != beta.shape:
-            raise ValueError(f"gamma and beta must be (channels,), got {tuple(gamma.shape)} and {tuple(beta.shape)}")
-        self.gamma, self.beta = gamma.requires_grad_(self.trainable), beta.requires_grad_(self.trainable)
+        with torch.inference_mode(False):  # tensors made in that mode could not train later
+            gamma, beta = (_lib.device_tensor(w, torch.float32).detach().clone() for w in weights)
+            if gamma.dim() != 1 or gamma.shape != beta.shape:
+                raise ValueError(f"gamma and beta must be (channels,), got {tuple(gamma.shape)} and {tuple(beta.shape)}")
+            self.gamma, self.beta = gamma.requires_grad_(self.trainable), beta.requires_grad_(self.trainable)
 
     def get_weights(self) -> List[torch.Tensor]:
         return [] if self.gamma is None else [self.gamma, self.beta]
@@ -99,6 +100,8 @@ class GroupNormalization(Layer):
     def call(self, inputs: torch.Tensor) -> torch.Tensor:
         """``(batch, ..., channels)`` -> the same shape and type."""
         if self.gamma is None:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{self.name}: call the layer once, or set its weights, before capturing it")
             channels, device = inputs.shape[-1], inputs.device if inputs.is_cuda else _lib.require_gpu()
             self.set_weights([torch.ones(channels, device=device), torch.zeros(channels, device=device)])
         return head_utils.group_norm(inputs, self.gamma, self.beta, self.groups, self.epsilon, self.activation)
@@ -108,7 +111,8 @@ class Dropout(Layer):
     """Dropout; every training call draws another mask from the layer's seed.
 
     The seed and the number of the call live in device memory and advance on the stream, so a captured training step draws
-    anew at each replay.  The first training call on a device makes that memory and may not itself be captured.
+    anew at each replay.  The first training call on a device makes that memory and may not itself be captured.  Calls of one
+    layer on several streams are for the caller to order, as with any tensor that a call updates.
     """
 
     def __init__(self, rate: float, seed: Optional[int] = None, **kwargs: Any) -> None:
@@ -135,7 +139,8 @@ class Dropout(Layer):
                 raise RuntimeError(f"{self.name}: call the layer once before capturing it")
             seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if self.seed is None else int(self.seed)
             seed = (seed + 2 ** 63) % 2 ** 64 - 2 ** 63  # the 64 bits as a signed integer
-            state = self._states[inputs.device] = torch.tensor([seed, 0], dtype=torch.int64, device=inputs.device)
+            with torch.inference_mode(False):  # a tensor made in that mode could not advance outside it
+                state = self._states[inputs.device] = torch.tensor([seed, 0], dtype=torch.int64, device=inputs.device)
         used = state.clone()
         state[1:].add_(1)
         return head_utils.dropout(inputs, self.rate, used)

@@ -285,7 +285,8 @@ def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
         x: ``(batch, ..., channels)`` fp32, fp16 or bf16 (a feature map ``(B, H, W, C)``, or pooled features with batch and
             proposals in one axis ``(B * R, 7, 7, C)``); made contiguous if it is not.
         gamma, beta: ``(channels,)``, used in fp32.
-        groups: divides the channels.
+        groups: divides the channels; of up to 512 channels each, or up to 512 times 16 bytes of them where a group is a whole
+            number of 16 bytes and the tensor is 16-byte aligned (others raise ``UnsupportedSizeError``).
         activation: ``None`` / ``"linear"``, ``"relu"`` or ``"swish"`` (``z / (1 + exp(-z))``).
         return_stats: also return ``stats (batch, groups, 2)`` fp32: mean and ``1 / sqrt(var + epsilon)``.
 
