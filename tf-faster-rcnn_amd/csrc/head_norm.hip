@@ -588,14 +588,51 @@ __global__ __launch_bounds__(256) void norm_grad_join_kernel(const float *__rest
   }
 }
 
+// dbeta[c], dgamma[c] = the sums of `parts` rows of (C, 2): 8 channels per block, THREADS / 16 threads down the rows of each.
+template <int THREADS>
+__device__ __forceinline__ void parameter_sums(int block, const float *__restrict__ sums, long long parts, int C, float *__restrict__ dgamma,
+                                               float *__restrict__ dbeta) {
+  constexpr int DOWN = THREADS / 16;
+  __shared__ float red[DOWN][17];
+  const int j = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const long long at = (long long)block * 16 + j;  // of 2 C
+  float s = 0.0f;
+  if (at < 2ll * C) {
+#pragma unroll 8
+    for (long long p = r; p < parts; p += DOWN) s += sums[p * 2 * C + at];
+  }
+  red[r][j] = s;
+  __syncthreads();
+  for (int half = DOWN / 2; half > 0; half >>= 1) {
+    if (r < half) red[r][j] += red[r + half][j];
+    __syncthreads();
+  }
+  if (r == 0 && at < 2ll * C) ((at & 1) ? dgamma : dbeta)[at >> 1] = red[0][j];
+}
+
+static unsigned parameter_blocks(int C) { return (unsigned)((2ll * C + 15) / 16); }
+
+__global__ __launch_bounds__(1024) void norm_grad_params_kernel(const float *__restrict__ sums, long long parts, int C,
+                                                                float *__restrict__ dgamma, float *__restrict__ dbeta) {
+  parameter_sums<1024>((int)blockIdx.x, sums, parts, C, dgamma, dbeta);
+}
+
+// dx; the first `param_blocks` workgroups add up the images' sums for dgamma and dbeta.
 template <typename T, int VEC, bool ONE>
 __global__ __launch_bounds__(512) void norm_grad_apply_kernel(const T *__restrict__ dy, const T *__restrict__ x,
                                                               const float *__restrict__ gamma, const float *__restrict__ beta,
                                                               const float *__restrict__ stats, const float *__restrict__ expect,
-                                                              T *__restrict__ dx, NormShape s, int act) {
+                                                              T *__restrict__ dx, const float *__restrict__ image_sums,
+                                                              float *__restrict__ dgamma, float *__restrict__ dbeta,
+                                                              unsigned param_blocks, NormShape s, int act) {
   using Gs = Groups<VEC, ONE>;
-  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
-  const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
+  if (blockIdx.x < param_blocks) {
+    parameter_sums<512>((int)blockIdx.x, image_sums, s.N, s.C, dgamma, dbeta);
+    return;
+  }
+  const unsigned block = blockIdx.x - param_blocks;
+  const int slab_index = (int)(block % (unsigned)s.slabs);
+  const int rest = (int)(block / (unsigned)s.slabs);
   const int chunk_index = rest % s.chunks, n = rest / s.chunks;
   const Column<VEC> me(s, slab_index);
   if (!me.active) return;
@@ -631,26 +668,6 @@ __global__ __launch_bounds__(512) void norm_grad_apply_kernel(const T *__restric
       }
     });
   });
-}
-
-// dbeta[c], dgamma[c] = the sums of `parts` rows of (C, 2): 8 channels per workgroup, 64 threads down the rows of each.
-__global__ __launch_bounds__(1024) void norm_grad_params_kernel(const float *__restrict__ sums, long long parts, int C,
-                                                                float *__restrict__ dgamma, float *__restrict__ dbeta) {
-  __shared__ float red[64][17];
-  const int j = threadIdx.x & 15, r = threadIdx.x >> 4;
-  const long long at = (long long)blockIdx.x * 16 + j;  // of 2 C
-  float s = 0.0f;
-  if (at < 2ll * C) {
-#pragma unroll 8
-    for (long long p = r; p < parts; p += 64) s += sums[p * 2 * C + at];
-  }
-  red[r][j] = s;
-  __syncthreads();
-  for (int half = 32; half > 0; half >>= 1) {
-    if (r < half) red[r][j] += red[r + half][j];
-    __syncthreads();
-  }
-  if (r == 0 && at < 2ll * C) ((at & 1) ? dgamma : dbeta)[at >> 1] = red[0][j];
 }
 
 // ---- the choice of a split -------------------------------------------------------------------------------------------------
@@ -818,14 +835,12 @@ static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, co
                             const float *stats, void *dx, float *dgamma, float *dbeta, float *workspace, int act,
                             hipStream_t stream) {
   const NormShape &s = p.s;
-  long long parts;
-  float *sums = workspace;
   int rc;
   if (p.resident) {
     const int per = grad_images_per_group(p);
-    parts = (s.N + per - 1) / per;
+    const long long parts = (s.N + per - 1) / per;
     auto resident = [&]() -> int {
-#define FRCNN_NORM_GRAD(NV) return launch_grad_resident<T, VEC, ONE, NV>(p, dy, x, gamma, beta, stats, dx, sums, per, parts, act, stream)
+#define FRCNN_NORM_GRAD(NV) return launch_grad_resident<T, VEC, ONE, NV>(p, dy, x, gamma, beta, stats, dx, workspace, per, parts, act, stream)
       switch (p.nv) {
         case 1: FRCNN_NORM_GRAD(1);
         case 4: FRCNN_NORM_GRAD(4);
@@ -843,11 +858,11 @@ static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, co
     };
     rc = resident();
     if (rc) return rc;
+    hipLaunchKernelGGL(norm_grad_params_kernel, dim3(parameter_blocks(s.C)), dim3(1024), 0, stream, workspace, parts, s.C, dgamma, dbeta);
+    return check_launch("group_norm_grad");
   } else {
-    parts = s.N;
     float *expect = workspace, *image_sums = expect + (size_t)s.N * s.G * 2;
     float *chunk_sums = image_sums + (size_t)s.N * s.C * 2;
-    sums = image_sums;
     const dim3 grid((unsigned)((long long)s.N * s.chunks * s.slabs));
     const size_t lds = 2 * (size_t)s.rows * s.slab * sizeof(float);
     rc = ensure_dynamic_lds((const void *)norm_grad_sums_kernel<T, VEC, ONE>, lds, "group_norm_grad");
@@ -860,14 +875,11 @@ static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, co
                        expect, s);
     rc = check_launch("group_norm_grad");
     if (rc) return rc;
-    hipLaunchKernelGGL((norm_grad_apply_kernel<T, VEC, ONE>), grid, dim3(p.threads), 0, stream, (const T *)dy, (const T *)x, gamma, beta,
-                       stats, expect, (T *)dx, s, act);
-    rc = check_launch("group_norm_grad");
-    if (rc) return rc;
+    const unsigned param_blocks = parameter_blocks(s.C);
+    hipLaunchKernelGGL((norm_grad_apply_kernel<T, VEC, ONE>), dim3(grid.x + param_blocks), dim3(p.threads), 0, stream, (const T *)dy,
+                       (const T *)x, gamma, beta, stats, expect, (T *)dx, image_sums, dgamma, dbeta, param_blocks, s, act);
+    return check_launch("group_norm_grad");
   }
-  hipLaunchKernelGGL(norm_grad_params_kernel, dim3((unsigned)((2ll * s.C + 15) / 16)), dim3(1024), 0, stream, sums, parts, s.C,
-                     dgamma, dbeta);
-  return check_launch("group_norm_grad");
 }
 
 // What the two entry points ask of a shape.
@@ -955,7 +967,7 @@ int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, in
   FRCNN_REQUIRE(aligned_to(dgamma, 4) && aligned_to(dbeta, 4), "group_norm_grad: misaligned pointer");
   hipStream_t st = (hipStream_t)stream;
   if (N == 0) {  // sums over nothing
-    hipLaunchKernelGGL(norm_grad_params_kernel, dim3((unsigned)((2ll * C + 15) / 16)), dim3(1024), 0, st, (const float *)nullptr, 0ll,
+    hipLaunchKernelGGL(norm_grad_params_kernel, dim3(parameter_blocks(C)), dim3(1024), 0, st, (const float *)nullptr, 0ll,
                        C, dgamma, dbeta);
     return check_launch("group_norm_grad");
   }
