@@ -335,6 +335,15 @@ def test_group_norm(head, shape, groups, dtype, activation):
     assert torch.equal(dx, again[0]) and torch.equal(dgamma, again[1]) and torch.equal(dbeta, again[2])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape,groups", [((9, 14, 14, 576), 32), ((1, 26, 26, 576), 32), ((2, 32, 32, 720), 24), ((5, 14, 14, 720), 24), ((3, 24, 24, 960), 32),
+                                          ((2, 33, 33, 36), 3), ((1, 9, 9, 1028), 4)])
+def test_group_norm_of_slabs_that_share_lines(head, shape, groups, dtype):
+    """Slabs whose rows begin and end inside lines of memory, on numbers of workgroups that the XCDs do not divide, and maps at the
+    limits of what a workgroup's registers hold."""
+    test_group_norm(head, shape, groups, dtype, "swish")
+
+
 @pytest.mark.parametrize("activation", [None, "swish"])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("shape,groups", [((1, 1, 8), 1), ((2, 5, 24), 3), ((3, 7, 7, 64), 32), ((2, 31, 31, 46), 2), ((1, 700, 1024), 1)])

@@ -88,4 +88,10 @@ struct Pack<T, 1> {
   __device__ __forceinline__ static void store(T *p, const float (&f)[1]) { *p = (T)f[0]; }
 };
 
+// Workgroups are dealt to the 8 XCDs in turn; this order gives each XCD a contiguous range of n places.
+__device__ __forceinline__ int xcd_contiguous(int i, int n) {
+  const int x = i & 7, base = n >> 3, more = n & 7;
+  return x * base + min(x, more) + (i >> 3);
+}
+
 }  // namespace frcnn

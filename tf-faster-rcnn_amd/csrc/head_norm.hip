@@ -73,6 +73,13 @@ struct NormShape {
   bool past;   // results are whole lines: stored past the caches
 };
 
+// The workgroup's place.  Slabs that share lines of memory run on one XCD, whose L2 joins their reads and writes: from all XCDs
+// (16, 1024, 576) fp32 in slabs of 144 bytes fetches 66 MB instead of 38, and takes 23.5 us instead of 18.6; (64, 196, 576) with
+// gradients 62.5 us instead of 53.5.  Where they share nothing this only costs: (8, 3969, 512) fp16 24.4 us to 25.3.
+__device__ __forceinline__ unsigned place_of(const NormShape &s) {
+  return s.past ? blockIdx.x : (unsigned)xcd_contiguous((int)blockIdx.x, (int)gridDim.x);
+}
+
 // ---- reductions inside a workgroup ---------------------------------------------------------------------------------------
 // red[rows][slab]: sum over the rows, into row 0.  `row` < rows are the threads that own data; halving keeps the order fixed.
 template <int VEC, int K>
@@ -203,8 +210,9 @@ __global__ __launch_bounds__(1024) void norm_resident_kernel(const T *__restrict
                                                            const float *__restrict__ beta, float *__restrict__ stats, NormShape s,
                                                            float eps, int act) {
   extern __shared__ float lds[];
-  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
-  const int rest = (int)(blockIdx.x / (unsigned)s.slabs);
+  const unsigned place = place_of(s);
+  const int slab_index = (int)(place % (unsigned)s.slabs);
+  const int rest = (int)(place / (unsigned)s.slabs);
   const int chunk_index = rest % s.chunks, n = rest / s.chunks;
   const Column<VEC> me(s, slab_index);
   const int c0 = slab_index * s.slab + me.col;
@@ -411,8 +419,9 @@ __global__ __launch_bounds__(512) void norm_grad_resident_kernel(const T *__rest
                                                                  float *__restrict__ sums, NormShape s, int per, int act) {
   extern __shared__ float lds[];
   using Gs = Groups<VEC, ONE>;
-  const int slab_index = (int)(blockIdx.x % (unsigned)s.slabs);
-  const int part = (int)(blockIdx.x / (unsigned)s.slabs);
+  const unsigned place = place_of(s);
+  const int slab_index = (int)(place % (unsigned)s.slabs);
+  const int part = (int)(place / (unsigned)s.slabs);
   const Column<VEC> me(s, slab_index);
   const int c0 = slab_index * s.slab + me.col;
   float *red = lds, *first = lds + 2 * me.rows * s.slab, *second = first + s.slab / s.Cg;
@@ -702,7 +711,7 @@ static int norm_threads(int columns, int S, int most, int limit) {
 }
 
 // Whole images per workgroup where a slab's packs fit its registers, chunks of positions otherwise.  grad: x and dz are held, in up
-// to 512 threads of 8 packs; the forward pass holds x, in up to 1024 threads of 16.
+// to 512 threads of 8 packs; the forward pass holds x, in up to 1024 threads of 16 (12 of 16-bit types).
 static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, bool grad) {
   NormPlan p = {};
   p.s.N = N, p.s.S = S, p.s.C = C, p.s.G = G, p.s.Cg = C / G;
@@ -723,7 +732,10 @@ static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, bo
   // overlap one's loads with another's sums, before large ones: (6000, 49, 512) bf16 forward 125 us with 256 threads and 142 with
   // 448, its gradients 207 and 229; not in
   // fp32, where a narrower slab's shorter rows cost more: (4800, 49, 576) forward 222 us against 204.
-  const int choices[3][2] = {{8, elem == 2 ? 256 : 0}, {8, 512}, {16, grad ? 0 : 1024}};
+  // What registers do not hold goes to chunks too: 16 packs of eight elements in 1024 threads spill ((16, 1024, 720) fp16 forward 57 us,
+  // 24 in chunks), and 512 threads of the gradients' 16-bit packs across groups take nearly all registers ((100, 196, 720) bf16
+  // 80 us, 64 in chunks; (2000, 196, 720) 1475 and 1050; (600, 196, 720) 305 and 317; others within 2 %; both with the forward call).
+  const int choices[3][2] = {{8, elem == 2 ? 256 : 0}, {8, grad && elem == 2 && !p.one ? 0 : 512}, {elem == 2 ? 12 : 16, grad ? 0 : 1024}};
   int most = 0, limit = 0;
   // the widest slab that fits; narrower ones while the chip is not full and a row is still a line
   long long k = widest;
@@ -789,8 +801,9 @@ static int launch_norm(const NormPlan &p, const void *x, void *y, const float *g
       case 1: FRCNN_NORM(1, true);
       case 4: FRCNN_NORM(4, true);
       case 8: FRCNN_NORM(8, true);
-      case 16: FRCNN_NORM(16, true);
     }
+    if constexpr (VEC == 1 || sizeof(T) == 4)
+      if (p.nv == 16) FRCNN_NORM(16, true);
     if constexpr (VEC > 1) switch (p.nv) {
       case 2: FRCNN_NORM(2, true);
       case 3: FRCNN_NORM(3, true);

@@ -277,13 +277,8 @@ struct TilePlan {
 
 static const int kStripRows = 4;
 
-// Workgroups are dealt to the 8 XCDs in turn: give each a contiguous range of the order, which runs down strips of kStripRows
-// row tiles, so that the 32 tiles an XCD works on share 4 rows' and 8 columns' operands in its L2.
-__device__ __forceinline__ int xcd_contiguous(int i, int n) {
-  const int x = i & 7, base = n >> 3, more = n & 7;
-  return x * base + min(x, more) + (i >> 3);
-}
-
+// Each XCD takes a contiguous range of an order that runs down strips of kStripRows row tiles, so that the 32 tiles it works on
+// share 4 rows' and 8 columns' operands in its L2.
 __device__ __forceinline__ void tile_of(const TilePlan &t, int order, int &m, int &n) {
   const int strip = order / (kStripRows * t.tiles_n), at = order - strip * kStripRows * t.tiles_n;
   const int rows = min(kStripRows, t.tiles_m - strip * kStripRows);
