@@ -763,7 +763,7 @@ static NormPlan norm_plan(int N, int S, int C, int G, int elem, bool aligned, bo
   p.s.slabs = (int)((units + k - 1) / k);
   p.s.rows = p.threads / (p.s.slab / vec);
   // Stores past the caches leave them to what is read: (16, 3969, 512) fp32 forward 81 us to 68, (1500, 49, 576) with gradients 187
-  // to 171.  Not where neighbouring workgroups share lines: (16, 1024, 576) in slabs of 144 bytes would take 38 us instead of 25.
+  // to 171.  Not where neighbouring workgroups share lines: (16, 1024, 576) in slabs of 144 bytes would take 29 us instead of 20.
   p.s.past = p.s.slabs == 1 || ((long long)p.s.slab * elem % kNormLine == 0 && (long long)C * elem % kNormLine == 0);
   if (!p.resident) {
     int per = 8;  // packs per thread and chunk; fewer while the chip is not full, at least four for a chunk's fixed costs
