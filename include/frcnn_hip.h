@@ -279,8 +279,9 @@ int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int rows, int K,
  * dot product of a's row m and b's row n, + bias[n]).  a (M, K) and b (N, K): e4m3, rows 16-byte aligned (row strides in
  * bytes, multiples of 16; nothing behind a row's K bytes is read); scales as frcnn_quantize_blocks leaves them with
  * block_rows 1 for a and 128 for b, both of scale_type.  bias (N) fp32 or NULL.  activation: none or relu.  Sums are held in
- * fp32.  K == 0 gives act(bias).  Limits: M <= 2^30, N <= 2^24, K <= 2^22, row strides
- * <= 2^23 bytes, ceil(M / 64) * ceil(N / 64) < 2^30. */
+ * fp32.  With y_type FRCNN_F32 or M <= 16 no product loses a bit; 16-bit results of more rows may come from the e4m3 matrix
+ * instructions, which cut the products of columns 8 i .. 8 i + 7 below 2^-13 of the largest of the eight.  K == 0 gives act(bias).
+ * Limits: M <= 2^30, N <= 2^24, K <= 2^22, row strides <= 2^23 bytes, ceil(M / 64) * ceil(N / 64) < 2^30. */
 size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K);
 int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_scale_row_stride,
                         int64_t a_scale_block_stride, const void *b, int64_t ldb, const void *b_scales,
