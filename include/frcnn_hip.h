@@ -271,7 +271,7 @@ int frcnn_roi_delta(const float *rois, const float *gt_boxes, const int32_t *gt_
  * become e4m3's NaN.  q (rows, K) has the row stride ldq, a multiple of 16, and starts at a multiple of 16 bytes; of each row
  * the bytes up to the next multiple of 16 are written (zeros behind K).  Scale (r / block_rows, kb) is written to
  * scales[(r / block_rows) * scale_row_stride + kb * scale_block_stride] (strides in elements). */
-int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int rows, int K, int block_rows, void *q, int64_t ldq,
+int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int64_t rows, int64_t K, int block_rows, void *q, int64_t ldq,
                           void *scales, int scale_type, int64_t scale_row_stride, int64_t scale_block_stride,
                           frcnn_stream_t stream);
 
@@ -282,11 +282,11 @@ int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int rows, int K,
  * fp32.  With y_type FRCNN_F32 or M <= 16 no product loses a bit; 16-bit results of more rows may come from the e4m3 matrix
  * instructions, which cut the products of columns 8 i .. 8 i + 7 below 2^-13 of the largest of the eight.  K == 0 gives act(bias).
  * Limits: M <= 2^30, N <= 2^24, K <= 2^22, row strides <= 2^23 bytes, ceil(M / 64) * ceil(N / 64) < 2^30. */
-size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K);
+size_t frcnn_scaled_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_scale_row_stride,
                         int64_t a_scale_block_stride, const void *b, int64_t ldb, const void *b_scales,
                         int64_t b_scale_row_stride, int64_t b_scale_block_stride, int scale_type, const float *bias,
-                        int activation, int M, int N, int K, void *y, int y_type, int64_t ldy, void *workspace,
+                        int activation, int64_t M, int64_t N, int64_t K, void *y, int y_type, int64_t ldy, void *workspace,
                         size_t workspace_bytes, frcnn_stream_t stream);
 
 /* Group normalisation of a channels-last tensor x (N, S, C) of `type`, C in G groups of neighbouring channels: mean and
@@ -294,14 +294,14 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
  * beta (C) fp32.  stats (N, G, 2) fp32, 8-byte aligned, receives mean and 1 / sqrt(var + epsilon) (NULL: not wanted).  S >= 1.  Groups of up
  * to 512 channels always, of up to 512 * 16 / sizeof(type) where 16 / sizeof(type) divides C / G and all rows are 16-byte
  * aligned. */
-size_t frcnn_group_norm_workspace_bytes(int type, int64_t N, int64_t S, int C, int G);
-int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int C, int G, const float *gamma, const float *beta,
+size_t frcnn_group_norm_workspace_bytes(int type, int64_t N, int64_t S, int64_t C, int64_t G);
+int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int64_t C, int64_t G, const float *gamma, const float *beta,
                      float epsilon, int activation, void *y, float *stats, void *workspace, size_t workspace_bytes,
                      frcnn_stream_t stream);
 /* Its gradients: dx of dy's type, dgamma and dbeta (C) fp32, from dy, x and the stats of the forward call.  Summed in a fixed
  * order: the same inputs give the same bits. */
-size_t frcnn_group_norm_grad_workspace_bytes(int type, int64_t N, int64_t S, int C, int G);
-int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, int64_t S, int C, int G, const float *gamma,
+size_t frcnn_group_norm_grad_workspace_bytes(int type, int64_t N, int64_t S, int64_t C, int64_t G);
+int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, int64_t S, int64_t C, int64_t G, const float *gamma,
                           const float *beta, const float *stats, int activation, void *dx, float *dgamma, float *dbeta,
                           void *workspace, size_t workspace_bytes, frcnn_stream_t stream);
 

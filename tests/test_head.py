@@ -129,3 +129,22 @@ def test_layer_configs_and_refusals():
         dense.set_weights([torch.zeros(4, 9)])
     x = torch.zeros(2)
     assert box.Dropout(0.5)(x) is x and box.Dropout(0.0)(x, training=True) is x
+
+
+@pytest.mark.parametrize("size", [2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 33 + 128, 2 ** 40])
+def test_sizes_beyond_32_bits_are_seen_whole(size):
+    """Counts reach the library in 64 bits: none of them is taken for its lower 32."""
+    big = -(-size // 128) * 128
+    refused(lib.frcnn_quantize_blocks(P, 0, 256, size, 256, 1, P, 256, P, 0, 1, 4, None), EUNSUPPORTED, b"%d" % size)
+    refused(lib.frcnn_quantize_blocks(P, 0, big, 4, big, 1, P, big, P, 0, 1, 4, None), EUNSUPPORTED, b"%d" % big)
+    refused(lib.frcnn_quantize_blocks(P, 0, big, 128, big, 128, P, big, P, 1, 1, 4, None), EUNSUPPORTED, b"%d" % big)
+    for m, n, k in ((size, 4, 256), (4, size, 256), (4, 4, big)):
+        ld = max(k, 256)
+        refused(lib.frcnn_scaled_matmul(P, ld, P, 1, 4, P, ld, P, 1, 1, 0, None, 0, m, n, k, P, 2, max(n, 4), None, 0, None), EUNSUPPORTED, b"index")
+        assert lib.frcnn_scaled_matmul_workspace_bytes(m, n, k) == 0
+    f = ctypes.c_float
+    for n, s, c, g in ((size, 49, 64, 8), (2, size, 64, 8), (2, 49, big, 8), (2, 50000, big + 64, big + 64)):
+        refused(lib.frcnn_group_norm(P, 0, n, s, c, g, P, P, f(1e-3), 0, P, None, P, 1 << 40, None), EUNSUPPORTED, b"index")
+        refused(lib.frcnn_group_norm_grad(P, P, 0, n, s, c, g, P, P, P, 0, P, P, P, P, 1 << 40, None), EUNSUPPORTED, b"index")
+        assert lib.frcnn_group_norm_workspace_bytes(0, n, s, c, g) == 0 and lib.frcnn_group_norm_grad_workspace_bytes(0, n, s, c, g) == 0
+    refused(lib.frcnn_group_norm(P, 0, 2, 49, 64, size, P, P, f(1e-3), 0, P, None, P, 1 << 40, None), EINVAL, b"multiple")

@@ -75,14 +75,14 @@ SIGNATURES: Dict[str, Tuple[Any, Sequence[Any]]] = {
     "frcnn_roi_delta_workspace_bytes": (_sz, [_i, _i, _i]),
     "frcnn_roi_delta": (_i, [_vp, _vp, _vp, _vp, _vp, ctypes.c_uint64, _i, _i, _i, _i, _i, _i, _c_float_p, _vp, _vp,
                              _vp, _sz, _vp]),
-    "frcnn_quantize_blocks": (_i, [_vp, _i, _i64, _i, _i, _i, _vp, _i64, _vp, _i, _i64, _i64, _vp]),
-    "frcnn_scaled_matmul_workspace_bytes": (_sz, [_i, _i, _i]),
-    "frcnn_scaled_matmul": (_i, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i, _vp, _i, _i, _i, _i, _vp, _i, _i64,
+    "frcnn_quantize_blocks": (_i, [_vp, _i, _i64, _i64, _i64, _i, _vp, _i64, _vp, _i, _i64, _i64, _vp]),
+    "frcnn_scaled_matmul_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "frcnn_scaled_matmul": (_i, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i, _vp, _i, _i64, _i64, _i64, _vp, _i, _i64,
                                  _vp, _sz, _vp]),
-    "frcnn_group_norm_workspace_bytes": (_sz, [_i, _i64, _i64, _i, _i]),
-    "frcnn_group_norm": (_i, [_vp, _i, _i64, _i64, _i, _i, _vp, _vp, _f, _i, _vp, _vp, _vp, _sz, _vp]),
-    "frcnn_group_norm_grad_workspace_bytes": (_sz, [_i, _i64, _i64, _i, _i]),
-    "frcnn_group_norm_grad": (_i, [_vp, _vp, _i, _i64, _i64, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "frcnn_group_norm_workspace_bytes": (_sz, [_i, _i64, _i64, _i64, _i64]),
+    "frcnn_group_norm": (_i, [_vp, _i, _i64, _i64, _i64, _i64, _vp, _vp, _f, _i, _vp, _vp, _vp, _sz, _vp]),
+    "frcnn_group_norm_grad_workspace_bytes": (_sz, [_i, _i64, _i64, _i64, _i64]),
+    "frcnn_group_norm_grad": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "frcnn_dropout": (_i, [_vp, _vp, _i, _i64, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _vp, _vp]),
 }
 

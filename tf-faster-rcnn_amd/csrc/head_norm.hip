@@ -896,13 +896,13 @@ static int launch_norm_grad(const NormPlan &p, const void *dy, const void *x, co
 }
 
 // What the two entry points ask of a shape.
-static int norm_check(const char *what, int type, int64_t N, int64_t S, int C, int G, int act) {
+static int norm_check(const char *what, int type, int64_t N, int64_t S, int64_t C, int64_t G, int act) {
   FRCNN_REQUIRE(type_known(type), "%s: unknown element type %d", what, type);
   FRCNN_REQUIRE(N >= 0 && S >= 1, "%s: needs at least one position per image (N=%lld, S=%lld)", what, (long long)N, (long long)S);
-  FRCNN_REQUIRE(C >= 1 && G >= 1 && C % G == 0, "%s: %d channels are not a multiple of %d groups", what, C, G);
+  FRCNN_REQUIRE(C >= 1 && G >= 1 && C % G == 0, "%s: %lld channels are not a multiple of %lld groups", what, (long long)C, (long long)G);
   FRCNN_REQUIRE(act == FRCNN_ACT_NONE || act == FRCNN_ACT_RELU || act == FRCNN_ACT_SWISH, "%s: unknown activation %d", what, act);
   if (N > (1ll << 30) || S >= (1ll << 24) || C > (1 << 20) || N * G >= (1ll << 31) || N * C >= (1ll << 38))
-    return set_error(FRCNN_EUNSUPPORTED, "%s: (%lld, %lld, %d) is beyond what the kernels index", what, (long long)N, (long long)S, C);
+    return set_error(FRCNN_EUNSUPPORTED, "%s: (%lld, %lld, %lld) is beyond what the kernels index", what, (long long)N, (long long)S, (long long)C);
   return FRCNN_OK;
 }
 
@@ -932,12 +932,12 @@ using namespace frcnn;
 
 extern "C" {
 
-size_t frcnn_group_norm_workspace_bytes(int type, int64_t N, int64_t S, int C, int G) {
+size_t frcnn_group_norm_workspace_bytes(int type, int64_t N, int64_t S, int64_t C, int64_t G) {
   if (norm_check("group_norm", type, N, S, C, G, FRCNN_ACT_NONE) || N == 0) return 0;
-  return norm_bytes((int)N, (int)S, C, G, (int)type_bytes(type), false);
+  return norm_bytes((int)N, (int)S, (int)C, (int)G, (int)type_bytes(type), false);
 }
 
-int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int C, int G, const float *gamma, const float *beta,
+int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int64_t C, int64_t G, const float *gamma, const float *beta,
                      float epsilon, int activation, void *y, float *stats, void *workspace, size_t workspace_bytes,
                      frcnn_stream_t stream) {
   const int bad = norm_check("group_norm", type, N, S, C, G, activation);
@@ -948,8 +948,8 @@ int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int C, int G
   const int elem = (int)type_bytes(type);
   FRCNN_REQUIRE(aligned_to(x, elem) && aligned_to(y, elem) && aligned_to(gamma, 4) && aligned_to(beta, 4) && aligned_to(stats, 8),
                 "group_norm: misaligned pointer");
-  const NormPlan p = norm_plan((int)N, (int)S, C, G, elem, aligned_to(x, 16) && aligned_to(y, 16), false);
-  if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm: %d channels per group", C / G);
+  const NormPlan p = norm_plan((int)N, (int)S, (int)C, (int)G, elem, aligned_to(x, 16) && aligned_to(y, 16), false);
+  if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm: %d channels per group", (int)(C / G));
   if ((long long)N * p.s.chunks * p.s.slabs >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "group_norm: too many workgroups");
   const size_t need = frcnn_group_norm_workspace_bytes(type, N, S, C, G);
   FRCNN_REQUIRE(need == 0 || (workspace && aligned_to(workspace, 256) && workspace_bytes >= need),
@@ -966,12 +966,12 @@ int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int C, int G
 #undef FRCNN_NORM_T
 }
 
-size_t frcnn_group_norm_grad_workspace_bytes(int type, int64_t N, int64_t S, int C, int G) {
+size_t frcnn_group_norm_grad_workspace_bytes(int type, int64_t N, int64_t S, int64_t C, int64_t G) {
   if (norm_check("group_norm_grad", type, N, S, C, G, FRCNN_ACT_NONE) || N == 0) return 0;
-  return norm_bytes((int)N, (int)S, C, G, (int)type_bytes(type), true);
+  return norm_bytes((int)N, (int)S, (int)C, (int)G, (int)type_bytes(type), true);
 }
 
-int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, int64_t S, int C, int G, const float *gamma,
+int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, int64_t S, int64_t C, int64_t G, const float *gamma,
                           const float *beta, const float *stats, int activation, void *dx, float *dgamma, float *dbeta,
                           void *workspace, size_t workspace_bytes, frcnn_stream_t stream) {
   const int bad = norm_check("group_norm_grad", type, N, S, C, G, activation);
@@ -980,8 +980,8 @@ int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, in
   FRCNN_REQUIRE(aligned_to(dgamma, 4) && aligned_to(dbeta, 4), "group_norm_grad: misaligned pointer");
   hipStream_t st = (hipStream_t)stream;
   if (N == 0) {  // sums over nothing
-    hipLaunchKernelGGL(norm_grad_params_kernel, dim3(parameter_blocks(C)), dim3(1024), 0, st, (const float *)nullptr, 0ll,
-                       C, dgamma, dbeta);
+    hipLaunchKernelGGL(norm_grad_params_kernel, dim3(parameter_blocks((int)C)), dim3(1024), 0, st, (const float *)nullptr, 0ll,
+                       (int)C, dgamma, dbeta);
     return check_launch("group_norm_grad");
   }
   FRCNN_REQUIRE(dy && x && gamma && beta && stats && dx, "group_norm_grad: null pointer");
@@ -989,8 +989,8 @@ int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, in
   FRCNN_REQUIRE(aligned_to(dy, elem) && aligned_to(x, elem) && aligned_to(dx, elem) && aligned_to(gamma, 4) && aligned_to(beta, 4) &&
                     aligned_to(stats, 8),
                 "group_norm_grad: misaligned pointer");
-  const NormPlan p = norm_plan((int)N, (int)S, C, G, elem, aligned_to(x, 16) && aligned_to(dy, 16) && aligned_to(dx, 16), true);
-  if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: %d channels per group", C / G);
+  const NormPlan p = norm_plan((int)N, (int)S, (int)C, (int)G, elem, aligned_to(x, 16) && aligned_to(dy, 16) && aligned_to(dx, 16), true);
+  if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: %d channels per group", (int)(C / G));
   if ((long long)N * p.s.chunks * p.s.slabs >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: too many workgroups");
   const size_t need = frcnn_group_norm_grad_workspace_bytes(type, N, S, C, G);
   FRCNN_REQUIRE(workspace && aligned_to(workspace, 256) && workspace_bytes >= need,

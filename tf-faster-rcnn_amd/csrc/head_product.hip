@@ -579,8 +579,8 @@ struct TileForm {
 static const TileForm kTileForms[] = {{256, 256, 1, 1.63f, 0.0f}, {160, 256, 1, 1.06f, 0.0f}, {128, 128, 2, 1.04f, 1.96f}, {64, 128, 2, 0.80f, 1.17f}};
 static const int kTileFormCount = sizeof(kTileForms) / sizeof(kTileForms[0]);
 
-static bool product_size_known(int M, int N, int K) {
-  return M <= (1 << 30) && N <= (1 << 24) && K <= (1 << 22) && (long long)((M + 63) / 64) * ((N + 63) / 64) < (1ll << 30);
+static bool product_size_known(int64_t M, int64_t N, int64_t K) {
+  return M <= (1 << 30) && N <= (1 << 24) && K <= (1 << 22) && (M + 63) / 64 * ((N + 63) / 64) < (1ll << 30);
 }
 
 static TilePlan tile_plan(const TileForm &f, int M, int N, int blocks) {
@@ -688,9 +688,9 @@ using namespace frcnn;
 
 extern "C" {
 
-size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K) {
-  if (M < 1 || N < 1 || K < 1 || !product_size_known(M, N, K)) return 0;
-  const int blocks = (K + kQuantBlock - 1) / kQuantBlock;
+size_t frcnn_scaled_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+  if (m < 1 || n < 1 || k < 1 || !product_size_known(m, n, k)) return 0;
+  const int M = (int)m, N = (int)n, blocks = (int)((k + kQuantBlock - 1) / kQuantBlock);
   size_t most = 0;
   for (int wide = 0; wide < 2; ++wide) {  // the output's type decides
     if (!use_tiles(M, N, blocks, wide != 0)) continue;
@@ -703,7 +703,7 @@ size_t frcnn_scaled_matmul_workspace_bytes(int M, int N, int K) {
 
 int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_scale_row_stride, int64_t a_scale_block_stride,
                         const void *b, int64_t ldb, const void *b_scales, int64_t b_scale_row_stride, int64_t b_scale_block_stride,
-                        int scale_type, const float *bias, int activation, int M, int N, int K, void *y, int y_type, int64_t ldy,
+                        int scale_type, const float *bias, int activation, int64_t M, int64_t N, int64_t K, void *y, int y_type, int64_t ldy,
                         void *workspace, size_t workspace_bytes, frcnn_stream_t stream) {
   FRCNN_REQUIRE(scale_type == FRCNN_SCALE_F32 || scale_type == FRCNN_SCALE_E8M0, "scaled_matmul: unknown scale type %d", scale_type);
   FRCNN_REQUIRE(type_known(y_type), "scaled_matmul: unknown output type %d", y_type);
@@ -721,15 +721,15 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
                   "scaled_matmul: negative scale stride");
   }
   if (!product_size_known(M, N, K) || lda > (1 << 23) || ldb > (1 << 23))
-    return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: M=%d, N=%d, K=%d (row strides %lld, %lld) is beyond what the kernels index", M, N, K,
-                     (long long)lda, (long long)ldb);
+    return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: M=%lld, N=%lld, K=%lld (row strides %lld, %lld) is beyond what the kernels index",
+                     (long long)M, (long long)N, (long long)K, (long long)lda, (long long)ldb);
   const size_t need = frcnn_scaled_matmul_workspace_bytes(M, N, K);
   FRCNN_REQUIRE(need == 0 || (workspace && aligned_to(workspace, 256) && workspace_bytes >= need),
                 "scaled_matmul: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);
   const int quads = N % 4 == 0 && ldy % 4 == 0 && aligned_to(y, 4 * type_bytes(y_type)) && aligned_to(bias, 16);
   const int rows16 = (ldy * (int64_t)type_bytes(y_type)) % 16 == 0 && aligned_to(y, 16);
   const ProductArgs p = {(const uint8_t *)a, (const uint8_t *)b, lda, ldb, a_scales, b_scales, a_scale_row_stride, a_scale_block_stride,
-                         b_scale_row_stride, b_scale_block_stride, bias, y, ldy, M, N, K, (K + kQuantBlock - 1) / kQuantBlock,
+                         b_scale_row_stride, b_scale_block_stride, bias, y, ldy, (int)M, (int)N, (int)K, (int)((K + kQuantBlock - 1) / kQuantBlock),
                          activation, y_type, quads, rows16};
   const int mode = (y_type == FRCNN_F32 ? kWideF32 : kNarrowF32) + (scale_type == FRCNN_SCALE_E8M0);
   hipStream_t s = (hipStream_t)stream;

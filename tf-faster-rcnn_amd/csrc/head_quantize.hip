@@ -151,7 +151,7 @@ static int launch_quantize(const void *x, long long ldx, int rows, int K, void *
 
 using namespace frcnn;
 
-extern "C" int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int rows, int K, int block_rows, void *q,
+extern "C" int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int64_t rows, int64_t K, int block_rows, void *q,
                                      int64_t ldq, void *scales, int scale_type, int64_t scale_row_stride,
                                      int64_t scale_block_stride, frcnn_stream_t stream) {
   FRCNN_REQUIRE(type_known(type), "quantize_blocks: unknown element type %d", type);
@@ -165,12 +165,13 @@ extern "C" int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int r
   FRCNN_REQUIRE(aligned_to(x, type_bytes(type)) && aligned_to(q, 16) && (scale_type == FRCNN_SCALE_E8M0 || aligned_to(scales, 4)),
                 "quantize_blocks: misaligned pointer");
   FRCNN_REQUIRE(scale_row_stride >= 0 && scale_block_stride >= 0, "quantize_blocks: negative scale stride");
-  FRCNN_REQUIRE(K <= (1 << 30), "quantize_blocks: rows longer than 2^30");
+  if (rows >= (1ll << 31) || K > (1 << 30))
+    return set_error(FRCNN_EUNSUPPORTED, "quantize_blocks: (%lld, %lld) is beyond what the kernels index", (long long)rows, (long long)K);
   const int p2 = scale_type == FRCNN_SCALE_E8M0;
   hipStream_t s = (hipStream_t)stream;
 #define FRCNN_QUANT(T)                                                                                                        \
-  (block_rows == 1 ? launch_quantize<T, 1>(x, ldx, rows, K, q, ldq, scales, scale_row_stride, scale_block_stride, p2, s)      \
-                   : launch_quantize<T, 128>(x, ldx, rows, K, q, ldq, scales, scale_row_stride, scale_block_stride, p2, s))
+  (block_rows == 1 ? launch_quantize<T, 1>(x, ldx, (int)rows, (int)K, q, ldq, scales, scale_row_stride, scale_block_stride, p2, s)      \
+                   : launch_quantize<T, 128>(x, ldx, (int)rows, (int)K, q, ldq, scales, scale_row_stride, scale_block_stride, p2, s))
   if (type == FRCNN_F32) return FRCNN_QUANT(float);
   if (type == FRCNN_F16) return FRCNN_QUANT(_Float16);
   return FRCNN_QUANT(__bf16);
