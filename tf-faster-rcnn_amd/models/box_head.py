@@ -20,8 +20,9 @@ from .faster_rcnn import Layer
 class QuantizedDense(Layer):
     """A Dense layer whose kernel is stored as e4m3 with a scale per 128 x 128 block, for inference.
 
-    The weights are quantised once, by ``set_weights``; a call quantises its input (a scale per row and 128 columns) and
-    multiplies.  Like the other inference layers it lets no gradient through: inputs that require one are refused.
+    The weights are taken once, by ``set_weights`` (the kernel quantised, the bias copied); a call quantises its input (a scale
+    per row and 128 columns) and multiplies.  Like the other inference layers it lets no gradient through: inputs that require
+    one are refused.
     """
 
     def __init__(self, units: int, activation: Optional[str] = None, scale_dtype: torch.dtype = torch.float32,
@@ -50,7 +51,7 @@ class QuantizedDense(Layer):
         device = kernel.device if kernel.is_cuda else _lib.require_gpu()
         bias = None
         if len(weights) == 2:
-            bias = _lib.device_tensor(weights[1], torch.float32, device).detach()
+            bias = _lib.device_tensor(weights[1], torch.float32, device).detach().clone()
             if tuple(bias.shape) != (self.units,):
                 raise ValueError(f"bias must be ({self.units},), got {tuple(bias.shape)}")
         rows = kernel.detach().to(device).t().contiguous()
