@@ -8,6 +8,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from tests import head_sums  # noqa: E402
+
 pytestmark = pytest.mark.gpu
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -76,3 +78,105 @@ def test_sums_of_blocks_are_fp32(head, knobs, form, out_dtype, scale_dtype):
         sa[:, 1] = 2.0 ** -t
         y = head.scaled_matmul(a.to(E4M3), sa.to(scale_dtype), b.to(E4M3), torch.ones((1, 3), device="cuda").to(scale_dtype), out_dtype=out_dtype)
         assert (y.float() == 2.0 ** -t).all(), t
+
+
+def operands(head, rows, units, inner, scale_dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((rows, inner), generator=g, device="cuda").clamp_min_(-0.3) * torch.exp2(torch.randn((rows, 1), generator=g, device="cuda"))
+    w = torch.randn((units, inner), generator=g, device="cuda") * inner ** -0.5
+    return (*head.quantize_blocks(x, scale_dtype=scale_dtype), *head.quantize_blocks(w, 128, scale_dtype=scale_dtype))
+
+
+def rows_of(a, sa, pick):
+    return a.view(torch.uint8)[pick].view(E4M3), sa.view(torch.uint8 if sa.dtype == E8M0 else sa.dtype)[pick].view(sa.dtype)
+
+
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+@pytest.mark.parametrize("out_dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,units,inner", [(1, 4096, 28224), (16, 1000, 25088), (300, 4096, 28224), (300, 105, 4096), (700, 520, 28230), (4800, 4096, 4100),
+                                              (2400, 1111, 2050), (64, 300, 130), (33, 129, 300000)])
+def test_sums_at_the_heads_sizes(head, rows, units, inner, out_dtype, scale_dtype):
+    """Within what the additions that there are may be off by: a lost chunk or a wrong scale in one of 221 blocks is seen."""
+    a, sa, b, sb = operands(head, rows, units, inner, scale_dtype, rows + inner)
+    bias = 0.1 * torch.randn((units,), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    y = head.scaled_matmul(a, sa, b, sb, bias=bias, out_dtype=out_dtype)
+    pick = torch.unique(torch.cat([torch.arange(0, rows, max(1, rows // 53), device="cuda"), torch.tensor([rows - 1], device="cuda")]))
+    want, l2 = head_sums.product(*rows_of(a, sa, pick), b, sb, bias)
+    allowed = head_sums.tolerance(want, l2, inner, out_dtype, out_dtype != F32 and rows > 16)
+    worst = ((y[pick].double() - want).abs() / allowed).max().item()
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("form", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+@pytest.mark.parametrize("rows,units,inner", [(40, 300, 128), (161, 257, 1000), (700, 1111, 2500), (300, 260, 28224)])
+def test_sums_of_every_form(head, knobs, rows, units, inner, scale_dtype, form):
+    knobs.setenv("FRCNN_PRODUCT_FORM", form)
+    a, sa, b, sb = operands(head, rows, units, inner, scale_dtype, form)
+    want, l2 = head_sums.product(a, sa, b, sb)
+    for out_dtype in (F32, F16, BF16):
+        y = head.scaled_matmul(a, sa, b, sb, out_dtype=out_dtype)
+        worst = ((y.double() - want).abs() / head_sums.tolerance(want, l2, inner, out_dtype, out_dtype != F32 and form != 4)).max().item()
+        assert worst <= 1, (out_dtype, worst)
+
+
+@pytest.mark.parametrize("form", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+@pytest.mark.parametrize("inner", [4096, 28224, 262144])
+def test_error_beneath_the_rounding(head, knobs, inner, scale_dtype, form):
+    """A bias of minus the sum leaves its error behind: neither the length of K nor the type of the scales makes it grow.  Also for
+    operands of one sign, where every cut has the same one: eight products lose less than 2^-13 of their largest each."""
+    knobs.setenv("FRCNN_PRODUCT_FORM", form)
+    for positive in (False, True):
+        g = torch.Generator(device="cuda").manual_seed(inner)
+        x, w = torch.randn((1, inner), generator=g, device="cuda"), torch.randn((200, inner), generator=g, device="cuda") * inner ** -0.5
+        if positive:
+            x, w = x.abs(), w.abs()
+        b, sb = head.quantize_blocks(w, 128, scale_dtype=scale_dtype)
+        a, sa = head.quantize_blocks(x.expand(40, inner), scale_dtype=scale_dtype)
+        sums, l2 = head_sums.product(*rows_of(a, sa, torch.zeros(1, dtype=torch.long, device="cuda")), b, sb)
+        bias = -sums[0].float()
+        for out_dtype in (F32, BF16):
+            y = head.scaled_matmul(a, sa, b, sb, bias=bias, out_dtype=out_dtype)
+            assert torch.equal(y, y[:1].expand_as(y))
+            left = (sums + bias.double())[0]
+            error = (y[0].double() - left).abs() - torch.finfo(out_dtype).eps / 2 * y[0].double().abs()
+            narrow = out_dtype != F32 and form != 4
+            if positive:
+                # the partial sums are the sum at most, each addition off by 2 U of it; an eight's largest product is its sum at most
+                allowed = sums[0] * (2 * head_sums.U * (inner // 128 + 64) + (7 * 2.0 ** -13 if narrow else 0))
+            else:
+                allowed = head_sums.tolerance(sums, l2, inner, F32, narrow)[0]
+            assert (error <= allowed).all(), (out_dtype, positive, (error / allowed).max().item())
+
+
+def test_parameter_gradients_of_many_images(head):
+    """dgamma and dbeta over 155000 pooled images, more than 2^32 elements, against sums in 64 bits.
+
+    dy = 2 relu(x) makes both sums ones of positive terms, of which a lost share is seen.  The kernel's threads (256 at least, 8
+    channels each) are about a thousand workgroups' worth, so a chain adds at most 1.25 * N S C / (1024 * 256 * 8) terms, and 200
+    join the chains; xhat is off by 160 U of (1 + mean / deviation) and itself."""
+    images, positions, channels, groups = 155000, 49, 576, 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty((images, positions, channels), dtype=BF16, device="cuda")
+    for i in range(0, images, 5000):
+        x[i:i + 5000].normal_(generator=g)
+    dy = x.clamp_min(0).mul_(2)
+    gamma, beta = torch.ones(channels, device="cuda"), torch.zeros(channels, device="cuda")
+    y, stats = head.group_norm(x, gamma, beta, groups, return_stats=True)
+    del y
+    _, dgamma, dbeta = head.group_norm_gradients(dy, x, gamma, beta, stats)
+    want_gamma, want_beta, size = (torch.zeros(channels, dtype=torch.float64, device="cuda") for _ in range(3))
+    for i in range(0, images, 1000):
+        v = x[i:i + 1000].double().view(1000, positions, groups, -1)
+        mean = v.mean((1, 3), keepdim=True)
+        centred = v - mean
+        xhat = (centred / torch.sqrt((centred * centred).mean((1, 3), keepdim=True) + 1e-3)).view(1000, positions, channels)
+        d = dy[i:i + 1000].double()
+        want_gamma += (d * xhat).sum((0, 1))
+        want_beta += d.sum((0, 1))
+        size += (d * xhat).abs().sum((0, 1))
+    depth = 1.25 * images * positions * channels / (1024 * 256 * 8) + 200
+    assert depth * head_sums.U < 2e-4  # a thousandth lost is seen
+    assert ((dbeta.double() - want_beta).abs() <= depth * head_sums.U * want_beta).all()
+    assert ((dgamma.double() - want_gamma).abs() <= (depth + 160) * head_sums.U * size + 160 * head_sums.U * 1.1 * want_beta).all()
