@@ -270,7 +270,8 @@ int frcnn_roi_delta(const float *rois, const float *gt_boxes, const int32_t *gt_
  * smallest power of two that is not below amax / 448, 2^-126 at least); q = x / scale rounded to nearest even.  NaN and infinities
  * become e4m3's NaN.  q (rows, K) has the row stride ldq, a multiple of 16, and starts at a multiple of 16 bytes; of each row
  * the bytes up to the next multiple of 16 are written (zeros behind K).  Scale (r / block_rows, kb) is written to
- * scales[(r / block_rows) * scale_row_stride + kb * scale_block_stride] (strides in elements). */
+ * scales[(r / block_rows) * scale_row_stride + kb * scale_block_stride] (strides in elements).  Limits: rows < 2^31, K <= 2^30,
+ * ceil(rows / 64) * ceil(K / 128) < 2^31. */
 int frcnn_quantize_blocks(const void *x, int type, int64_t ldx, int64_t rows, int64_t K, int block_rows, void *q, int64_t ldq,
                           void *scales, int scale_type, int64_t scale_row_stride, int64_t scale_block_stride,
                           frcnn_stream_t stream);
@@ -293,7 +294,8 @@ int frcnn_scaled_matmul(const void *a, int64_t lda, const void *a_scales, int64_
  * variance per image and group over S * (C / G) values, y = act((x - mean) / sqrt(var + epsilon) * gamma + beta).  gamma,
  * beta (C) fp32.  stats (N, G, 2) fp32, 8-byte aligned, receives mean and 1 / sqrt(var + epsilon) (NULL: not wanted).  S >= 1.  Groups of up
  * to 512 channels always, of up to 512 * 16 / sizeof(type) where 16 / sizeof(type) divides C / G and all rows are 16-byte
- * aligned. */
+ * aligned.  Limits: N <= 2^30, S < 2^24, C <= 2^20, N G < 2^31.  Images that are cut into chunks (of 2048 elements at least):
+ * fewer than 2^23 chunks an image, for the gradients fewer than 2^22 in all and N G < 2^24. */
 size_t frcnn_group_norm_workspace_bytes(int type, int64_t N, int64_t S, int64_t C, int64_t G);
 int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int64_t C, int64_t G, const float *gamma, const float *beta,
                      float epsilon, int activation, void *y, float *stats, void *workspace, size_t workspace_bytes,

@@ -19,6 +19,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 static const int kQuantBlock = 128;          // elements per scale along a row
 static const float kE4M3Max = 448.0f;        // largest finite e4m3
 
+static const long long kGridThreads = (1ll << 32) - 1;  // threads of one launch at most
+
 static inline size_t type_bytes(int type) { return type == FRCNN_F32 ? 4 : 2; }
 static inline bool type_known(int type) { return type == FRCNN_F32 || type == FRCNN_F16 || type == FRCNN_BF16; }
 

@@ -950,20 +950,30 @@ int frcnn_group_norm(const void *x, int type, int64_t N, int64_t S, int64_t C, i
                 "group_norm: misaligned pointer");
   const NormPlan p = norm_plan((int)N, (int)S, (int)C, (int)G, elem, aligned_to(x, 16) && aligned_to(y, 16), false);
   if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm: %d channels per group", (int)(C / G));
-  if ((long long)N * p.s.chunks * p.s.slabs >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "group_norm: too many workgroups");
+  // images of one launch: workgroups of p.threads, and a wave per group in norm_join_kernel, whose workgroups have four
+  const long long threads = (long long)p.s.chunks * p.s.slabs * p.threads, joins = 64ll * G;
+  const long long most = (kGridThreads - 255) / (threads > joins ? threads : joins);
+  if (most < 1) return set_error(FRCNN_EUNSUPPORTED, "group_norm: (%lld, %lld, %lld) takes too many threads", (long long)N, (long long)S, (long long)C);
   const size_t need = frcnn_group_norm_workspace_bytes(type, N, S, C, G);
   FRCNN_REQUIRE(need == 0 || (workspace && aligned_to(workspace, 256) && workspace_bytes >= need),
                 "group_norm: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);
   hipStream_t st = (hipStream_t)stream;
   float *ws = (float *)workspace;
-#define FRCNN_NORM_T(T)                                                                                       \
-  (p.vec == 1 ? launch_norm<T, 1, true>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st)                        \
-   : p.one    ? launch_norm<T, 16 / sizeof(T), true>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st)          \
-              : launch_norm<T, 16 / sizeof(T), false>(p, x, y, gamma, beta, stats, ws, epsilon, activation, st))
-  if (type == FRCNN_F32) return FRCNN_NORM_T(float);
-  if (type == FRCNN_F16) return FRCNN_NORM_T(_Float16);
-  return FRCNN_NORM_T(__bf16);
+  for (int64_t first = 0; first < N; first += most) {
+    NormPlan part = p;
+    part.s.N = (int)(N - first < most ? N - first : most);
+    const void *from = (const uint8_t *)x + first * S * C * elem;
+    void *to = (uint8_t *)y + first * S * C * elem;
+    float *out = stats ? stats + first * G * 2 : nullptr;
+#define FRCNN_NORM_T(T)                                                                                                \
+  (p.vec == 1 ? launch_norm<T, 1, true>(part, from, to, gamma, beta, out, ws, epsilon, activation, st)                \
+   : p.one    ? launch_norm<T, 16 / sizeof(T), true>(part, from, to, gamma, beta, out, ws, epsilon, activation, st)   \
+              : launch_norm<T, 16 / sizeof(T), false>(part, from, to, gamma, beta, out, ws, epsilon, activation, st))
+    const int rc = type == FRCNN_F32 ? FRCNN_NORM_T(float) : type == FRCNN_F16 ? FRCNN_NORM_T(_Float16) : FRCNN_NORM_T(__bf16);
 #undef FRCNN_NORM_T
+    if (rc) return rc;
+  }
+  return FRCNN_OK;
 }
 
 size_t frcnn_group_norm_grad_workspace_bytes(int type, int64_t N, int64_t S, int64_t C, int64_t G) {
@@ -991,7 +1001,9 @@ int frcnn_group_norm_grad(const void *dy, const void *x, int type, int64_t N, in
                 "group_norm_grad: misaligned pointer");
   const NormPlan p = norm_plan((int)N, (int)S, (int)C, (int)G, elem, aligned_to(x, 16) && aligned_to(dy, 16) && aligned_to(dx, 16), true);
   if (!p.vec) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: %d channels per group", (int)(C / G));
-  if ((long long)N * p.s.chunks * p.s.slabs >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: too many workgroups");
+  // the form that keeps images in registers takes about a thousand workgroups; the others one per chunk and per group
+  if (!p.resident && ((long long)N * p.s.chunks * p.s.slabs + parameter_blocks((int)C) > kGridThreads / 512 || N * G > kGridThreads / 256))
+    return set_error(FRCNN_EUNSUPPORTED, "group_norm_grad: (%lld, %lld, %lld) takes too many threads", (long long)N, (long long)S, (long long)C);
   const size_t need = frcnn_group_norm_grad_workspace_bytes(type, N, S, C, G);
   FRCNN_REQUIRE(workspace && aligned_to(workspace, 256) && workspace_bytes >= need,
                 "group_norm_grad: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, workspace_bytes);

@@ -583,6 +583,11 @@ static bool product_size_known(int64_t M, int64_t N, int64_t K) {
   return M <= (1 << 30) && N <= (1 << 24) && K <= (1 << 22) && (M + 63) / 64 * ((N + 63) / 64) < (1ll << 30);
 }
 
+// One launch holds the form's tiles, 512 threads each, and the pieces of a round of them.
+static bool form_fits(const TileForm &f, int M, int N) {
+  return (((long long)M + f.bm - 1) / f.bm) * (((long long)N + f.bn - 1) / f.bn) <= kGridThreads / 512 - kProductCus * f.per_cu;
+}
+
 static TilePlan tile_plan(const TileForm &f, int M, int N, int blocks) {
   TilePlan t;
   t.tiles_m = (M + f.bm - 1) / f.bm;
@@ -626,10 +631,11 @@ static int best_form(int M, int N, int blocks, bool wide) {
 // A workgroup of product_split_kernel streams 4 KB per 16 x 16 tile and block through the chip at about 7.5 TB/s.
 static bool use_tiles(int M, int N, int blocks, bool wide) {
   if (blocks == 0) return false;
+  const TileForm &f = kTileForms[best_form(M, N, blocks, wide)];
+  if (!form_fits(f, M, N)) return false;
   const int forced = knob(kKnobProductForm, -1);
   if (forced >= 0) return forced < kTileFormCount;
   if (M <= 16) return false;
-  const TileForm &f = kTileForms[best_form(M, N, blocks, wide)];
   const double split_us = 4.0 + (double)((M + 15) / 16) * ((N + 15) / 16) * blocks * 5.5e-4;
   return plan_us(f, tile_plan(f, M, N, blocks), blocks, wide) < split_us;
 }
@@ -670,10 +676,20 @@ static int launch_tiles(const ProductArgs &p, void *workspace, size_t workspace_
 
 template <int TM, int TN, int W, int MODE>
 static int launch_split(const ProductArgs &p, hipStream_t s) {
-  const long long tm = (p.M + TM * 16 - 1) / (TM * 16), tn = (p.N + TN * 16 - 1) / (TN * 16);
-  if (tm * tn >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "scaled_matmul: too many tiles");
-  hipLaunchKernelGGL((product_split_kernel<TM, TN, W, MODE>), dim3((unsigned)(tm * tn)), dim3(64 * W), 0, s, p, (int)tn);
-  return check_launch("scaled_matmul");
+  const long long tn = ((long long)p.N + TN * 16 - 1) / (TN * 16);
+  const long long most = kGridThreads / (64 * W) / tn * (TM * 16);  // rows of one launch; N <= 2^24 leaves some
+  for (long long first = 0; first < p.M; first += most) {
+    ProductArgs part = p;
+    part.M = (int)(p.M - first < most ? p.M - first : most);
+    part.a += first * p.lda;
+    part.sa = (const uint8_t *)p.sa + first * p.sa_row * (MODE == kNarrowE8M0 || MODE == kWideE8M0 ? 1 : 4);
+    part.y = (uint8_t *)p.y + first * p.ldy * (long long)type_bytes(p.out);
+    const long long tm = ((long long)part.M + TM * 16 - 1) / (TM * 16);
+    hipLaunchKernelGGL((product_split_kernel<TM, TN, W, MODE>), dim3((unsigned)(tm * tn)), dim3(64 * W), 0, s, part, (int)tn);
+    const int rc = check_launch("scaled_matmul");
+    if (rc) return rc;
+  }
+  return FRCNN_OK;
 }
 
 template <int MODE>

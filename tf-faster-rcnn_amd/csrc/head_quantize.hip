@@ -135,16 +135,25 @@ static int launch_quantize(const void *x, long long ldx, int rows, int K, void *
                            long long scale_row, long long scale_block, int power_of_two, hipStream_t stream) {
   const int across = (K + kQuantBlock - 1) / kQuantBlock;
   const int per = BR == 1 ? 64 : 128;
-  const long long blocks = ((long long)rows + per - 1) / per * across;
-  if (blocks >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "quantize_blocks: too many blocks");
+  if (((long long)rows + per - 1) / per * across >= (1ll << 31)) return set_error(FRCNN_EUNSUPPORTED, "quantize_blocks: too many blocks");
   const bool vector = aligned_to(x, 16) && (ldx * (long long)sizeof(T)) % 16 == 0;
-  if (vector)
-    hipLaunchKernelGGL((quantize_kernel<T, true, BR>), dim3((unsigned)blocks), dim3(256), 0, stream, (const T *)x, ldx, rows, K,
-                       (uint8_t *)q, ldq, scales, scale_row, scale_block, power_of_two, across);
-  else
-    hipLaunchKernelGGL((quantize_kernel<T, false, BR>), dim3((unsigned)blocks), dim3(256), 0, stream, (const T *)x, ldx, rows,
-                       K, (uint8_t *)q, ldq, scales, scale_row, scale_block, power_of_two, across);
-  return check_launch("quantize_blocks");
+  const long long most = kGridThreads / 256 / across * per;  // rows of one launch
+  for (long long first = 0; first < rows; first += most) {
+    const int count = (int)(rows - first < most ? rows - first : most);
+    const dim3 grid((unsigned)(((long long)count + per - 1) / per * across));
+    const T *from = (const T *)x + first * ldx;
+    uint8_t *to = (uint8_t *)q + first * ldq;
+    void *s = (uint8_t *)scales + first / BR * scale_row * (power_of_two ? 1 : 4);
+    if (vector)
+      hipLaunchKernelGGL((quantize_kernel<T, true, BR>), grid, dim3(256), 0, stream, from, ldx, count, K, to, ldq, s, scale_row, scale_block,
+                         power_of_two, across);
+    else
+      hipLaunchKernelGGL((quantize_kernel<T, false, BR>), grid, dim3(256), 0, stream, from, ldx, count, K, to, ldq, s, scale_row, scale_block,
+                         power_of_two, across);
+    const int rc = check_launch("quantize_blocks");
+    if (rc) return rc;
+  }
+  return FRCNN_OK;
 }
 
 }  // namespace frcnn
