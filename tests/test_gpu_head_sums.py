@@ -180,3 +180,63 @@ def test_parameter_gradients_of_many_images(head):
     assert depth * head_sums.U < 2e-4  # a thousandth lost is seen
     assert ((dbeta.double() - want_beta).abs() <= depth * head_sums.U * want_beta).all()
     assert ((dgamma.double() - want_gamma).abs() <= (depth + 160) * head_sums.U * size + 160 * head_sums.U * 1.1 * want_beta).all()
+
+
+@pytest.mark.parametrize("form", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+@pytest.mark.parametrize("inner", [384, 640, 1250])
+@pytest.mark.parametrize("far", [(100, 30), (-100, -30), (-120, -32), (120, 7), (20, 107), (-126, -1)])
+def test_products_of_scales_beyond_fp32(head, knobs, far, inner, scale_dtype, form):
+    """Scales whose product is no fp32 number while the result is one, in some rows' second block: a block of zeros gives zero, the
+    smallest sum 2^-18 and the largest 2^24.6 what they are worth; other rows and blocks are as ever."""
+    knobs.setenv("FRCNN_PRODUCT_FORM", form)
+    ea, eb = far
+    rows, units = 70, 200
+    blocks = -(-inner // 128)
+    a, b = torch.ones((rows, inner), device="cuda"), torch.ones((units, inner), device="cuda")
+    a[3::5, 128:256], b[:, 128:256] = 0.0, 0.0
+    b[:, 128] = 2.0 ** -9
+    a[0::5, 128:256] = 2.0 ** -9  # sums of 2^-18
+    if ea + eb < 0:
+        a[0::5, 128:256], b[:, 128:256] = 448.0, 448.0
+    # others: 0 in the far block
+    a[1::5, 128:256], a[2::5, 128:256], a[4::5, 128:256] = 0.0, 0.0, 0.0
+    a, b = a.to(E4M3), b.to(E4M3)
+    step = 1.0 if scale_dtype == E8M0 else 1.375
+    sa, sb = torch.ones((rows, blocks), device="cuda"), torch.ones((2, blocks), device="cuda")
+    sa[0::5, 1], sa[3::5, 1], sb[:, 1] = step * 2.0 ** ea, step * 2.0 ** ea, step * 2.0 ** eb
+    if ea + eb < 0:
+        sa[0::5, ::2] = 0.0 if scale_dtype == F32 else 2.0 ** -127
+        sa[0::5, 3::2] = sa[0::5, :1]
+    sa, sb = sa.to(scale_dtype), sb.to(scale_dtype)
+    want, _ = head_sums.product(a, sa, b, sb)
+    if ea + eb < 0 and scale_dtype == E8M0:  # the other blocks' 2^-127 are beside the far block's 2^-106 and more
+        assert want[0, 0] > 2.0 ** -127
+    for out_dtype in (F32, BF16):
+        y = head.scaled_matmul(a, sa, b, sb, out_dtype=out_dtype)
+        # all terms are positive: the roundings of the sums and of the scales, and the type's own; where the result is subnormal,
+        # half of the type's smallest step, and a step of fp32's for each block
+        half = torch.finfo(out_dtype).eps / 2
+        off = (half + (blocks + 8) * 2 * head_sums.U) * want.abs() + half * 2.0 ** -126 + 2.0 ** -149 * blocks
+        assert torch.isfinite(y).all()
+        assert ((y.double() - want).abs() <= off).all(), (out_dtype, ((y.double() - want).abs() / off).max().item())
+
+
+@pytest.mark.parametrize("form", [0, 2, 4])
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+def test_scales_that_are_no_numbers(head, knobs, out_dtype, form):
+    """Infinite and NaN scales reach what they scale and nothing else; a zero scale makes zeros."""
+    knobs.setenv("FRCNN_PRODUCT_FORM", form)
+    a, b = torch.ones((40, 300), device="cuda"), torch.ones((260, 300), device="cuda")
+    a[7, 128:256] = 0.0
+    sa, sb = torch.ones((40, 3), device="cuda"), torch.ones((3, 3), device="cuda")
+    sa[5, 1], sa[6, 2], sa[7, 1], sa[8] = float("inf"), float("nan"), float("inf"), 0.0
+    sb[1, 0] = float("inf")
+    y = head.scaled_matmul(a.to(E4M3), sa, b.to(E4M3), sb, out_dtype=out_dtype).float()
+    want = torch.full((40, 260), 300.0, device="cuda")
+    want[:, 128:256] = float("inf")
+    want[5], want[6], want[7] = float("inf"), float("nan"), float("nan")  # 0 times infinity
+    want[8] = 0.0
+    want[8, 128:256] = float("nan")
+    want = want.to(out_dtype).float()
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.nan_to_num(y, nan=1.0), torch.nan_to_num(want, nan=1.0))

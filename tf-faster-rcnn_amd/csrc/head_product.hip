@@ -126,13 +126,18 @@ __device__ __forceinline__ void add_scaled(f32x4 &acc, f32x4 d, float s) {
   for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
 }
 
-template <int MODE>
-__device__ __forceinline__ void multiply(const typename Operand<MODE>::type &w, const typename Operand<MODE>::type &a, f32x4 &acc,
-                                         typename Scale<MODE>::type sw, typename Scale<MODE>::type sa) {
-  if constexpr (MODE == kNarrowE8M0)
-    acc = block_product<MODE>(w, a, acc, sw, sa);
-  else
-    add_scaled(acc, block_product<MODE>(w, a, f32x4{0, 0, 0, 0}, sw, sa), sw * sa);
+// Is the product of two scales no normal number, other than for a zero among them?  Times a block's sum (2^-18 to 2^25) it may be one.
+__device__ __forceinline__ bool far_scales(float sw, float sa) {
+  const float f = sw * sa;
+  return __builtin_amdgcn_classf(f, 0x297) || (f == 0.0f && sw != 0.0f && sa != 0.0f);  // NaN, infinity, subnormal; vanished
+}
+
+// acc + d sw sa for such scales: their powers of two are applied last.
+__device__ __forceinline__ void add_far_scaled(f32x4 &acc, f32x4 d, float sw, float sa) {
+  const float m = __builtin_amdgcn_frexp_mantf(sw) * __builtin_amdgcn_frexp_mantf(sa);
+  const int e = __builtin_amdgcn_frexp_expf(sw) + __builtin_amdgcn_frexp_expf(sa);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] += __builtin_amdgcn_ldexpf(d[i] * m, e);
 }
 
 __device__ __forceinline__ float relu(float v) { return v > 0.0f ? v : (v != v ? v : 0.0f); }
@@ -246,7 +251,14 @@ __global__ __launch_bounds__(64 * W) void product_split_kernel(ProductArgs p, in
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) multiply<MODE>(b[j], a[i], acc[i][j], sb[j], sa[i]);
+      for (int j = 0; j < TN; ++j) {
+        const f32x4 d = block_product<MODE>(b[j], a[i], f32x4{0, 0, 0, 0}, sb[j], sa[i]);
+        const float both = sb[j] * sa[i];
+        if (__builtin_expect(__any(__builtin_amdgcn_classf(both, 0x2F7)), 0) && far_scales(sb[j], sa[i]))  // no normal number
+          add_far_scaled(acc[i][j], d, sb[j], sa[i]);
+        else
+          add_scaled(acc[i][j], d, both);
+      }
   }
   __shared__ f32x4 part[W][TM * TN][64];
 #pragma unroll
@@ -418,12 +430,32 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
     for (int i = 0; i < SCALES; ++i) sa_next[i] = S::load(p.sa, sa_at[i] + block * p.sa_block);
     sb_next = S::load(p.sb, sb_at + block * p.sb_block);
   };
-  // The lane's scale of row i * 16 + lane % 16 for every i, and b's scale
+  // For row i * 16 + lane % 16 and every i: what the instruction takes, a's scale, with b's beside it; otherwise the product of the two
   typename S::type sa[SCALES * 4], sb;
+  uint64_t far = 0;  // not zero: rows whose scales are far from 1 were left out (times 0), and come last
   auto take_scales = [&]() {
+    if constexpr (MODE == kNarrowE8M0) {
+      sb = sb_next;
 #pragma unroll
-    for (int i = 0; i < SCALES; ++i) rows_of_16_to_all(sa_next[i], sa + 4 * i);
-    sb = sb_next;
+      for (int i = 0; i < SCALES; ++i) rows_of_16_to_all(sa_next[i], sa + 4 * i);
+    } else {
+      float both[SCALES];
+      uint64_t odd = 0;
+#pragma unroll
+      for (int i = 0; i < SCALES; ++i) {
+        both[i] = sb_next * sa_next[i];
+        odd |= __builtin_amdgcn_ballot_w64(__builtin_amdgcn_classf(both[i], 0x2F7));  // no normal number
+      }
+      if (__builtin_expect(odd != 0, 0))
+#pragma unroll
+        for (int i = 0; i < SCALES; ++i) {
+          const bool f = far_scales(sb_next, sa_next[i]);
+          far |= __builtin_amdgcn_ballot_w64(f);
+          both[i] = f ? 0.0f : both[i];
+        }
+#pragma unroll
+      for (int i = 0; i < SCALES; ++i) rows_of_16_to_all(both[i], sa + 4 * i);
+    }
   };
   const int lane_at = (lane & 15) * kQuantBlock + (((lane >> 4) ^ (lane & 7)) << 4);
   // a's next operand is read while this one is multiplied, and a group's scaled sums follow the next group's products
@@ -451,7 +483,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
       if constexpr (MODE != kNarrowE8M0) {
         if (i > 0)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) add_scaled(acc[i - 1][j], before[j], sb * sa[i - 1]);
+          for (int j = 0; j < NT; ++j) add_scaled(acc[i - 1][j], before[j], sa[i - 1]);
 #pragma unroll
         for (int j = 0; j < NT; ++j) before[j] = now[j];
       }
@@ -460,7 +492,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
     }
     if constexpr (MODE != kNarrowE8M0)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) add_scaled(acc[MT - 1][j], before[j], sb * sa[MT - 1]);
+      for (int j = 0; j < NT; ++j) add_scaled(acc[MT - 1][j], before[j], sa[MT - 1]);
   };
   constexpr int A = BM * kQuantBlock, B = BN * kQuantBlock;
   uint8_t *const bs = smem + 3 * A;
@@ -506,6 +538,30 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN * PER_CU / 4) void product_ti
     compute(smem, bs, [](int) {});
     step_barrier<0>();  // LDS is free for the results
   }
+  if constexpr (MODE != kNarrowE8M0)
+    if (far) {
+#pragma unroll 1
+      for (int kb = k0; kb < k1; ++kb) {
+        const float sw = S::load(p.sb, sb_at + kb * p.sb_block);
+        int row = lane & 15;  // seen as new in each block: addresses kept over the loop would take registers that the sums need
+        asm volatile("" : "+v"(row));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int m = min(m0 + wm + i * 16 + row, p.M - 1);
+          const float sv = S::load(p.sa, m * p.sa_row + kb * p.sa_block);
+          const bool mine = far_scales(sw, sv);
+          if (!__any(mine)) continue;
+          const typename O::type v = O::of(load_operand(p.a + m * p.lda, kb, p.K));
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const int n = min(n0 + wn + j * 16 + row, p.N - 1);
+            const f32x4 d = block_product<MODE>(O::of(load_operand(p.b + n * p.ldb, kb, p.K)), v, f32x4{0, 0, 0, 0}, sw, sv);
+            if (mine) add_far_scaled(acc[i][j], d, sw, sv);
+            __builtin_amdgcn_sched_barrier(0);  // few registers beside the sums
+          }
+        }
+      }
+    }
   if (piece >= 0) {
     f32x4 *out = partial + (long long)piece * (MT * NT * THREADS) + threadIdx.x;
 #pragma unroll
