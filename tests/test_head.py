@@ -148,3 +148,36 @@ def test_sizes_beyond_32_bits_are_seen_whole(size):
         refused(lib.frcnn_group_norm_grad(P, P, 0, n, s, c, g, P, P, P, 0, P, P, P, P, 1 << 40, None), EUNSUPPORTED, b"index")
         assert lib.frcnn_group_norm_workspace_bytes(0, n, s, c, g) == 0 and lib.frcnn_group_norm_grad_workspace_bytes(0, n, s, c, g) == 0
     refused(lib.frcnn_group_norm(P, 0, 2, 49, 64, size, P, P, f(1e-3), 0, P, None, P, 1 << 40, None), EINVAL, b"multiple")
+
+
+def calls_on(x, gamma):
+    """Each operator with `x` in the place of every tensor that has derivatives, and of `gamma` alone."""
+    h = pkg.head_utils
+    plain, ones = torch.ones(2, 3, 8), torch.ones(8)
+    stats = torch.ones(2, 2, 2)
+    a = torch.zeros(2, 8, dtype=torch.float8_e4m3fn)
+    one = torch.ones(2, 1)
+    return {"group_norm": [lambda: h.group_norm(x, ones, ones, 2), lambda: h.group_norm(plain, gamma, ones, 2), lambda: h.group_norm(plain, ones, gamma, 2)],
+            "group_norm_gradients": [lambda: h.group_norm_gradients(x, plain, ones, ones, stats), lambda: h.group_norm_gradients(plain, x, ones, ones, stats),
+                                     lambda: h.group_norm_gradients(plain, plain, gamma, ones, stats)],
+            "dropout": [lambda: h.dropout(x, 0.5, 1)],
+            "quantize_blocks": [lambda: h.quantize_blocks(x)],
+            "scaled_matmul": [lambda: h.scaled_matmul(a, one, a, one[:1], bias=gamma)]}
+
+
+@pytest.mark.parametrize("operator", ["group_norm", "group_norm_gradients", "dropout", "quantize_blocks", "scaled_matmul"])
+def test_forward_mode_derivatives_and_traces_are_refused(operator):
+    """They would come back without a tangent, that is with derivative zero, or as a record of uninitialised memory."""
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in calls_on(dual(torch.ones(2, 3, 8)), dual(torch.ones(8)))[operator]:
+            with pytest.raises(RuntimeError, match=f"{operator} has no forward-mode"):
+                call()
+    for at in range(len(calls_on(None, None)[operator])):
+        def traced(x, gamma):
+            calls_on(x, gamma)[operator][at]()
+            return x
+        with pytest.raises(RuntimeError, match=f"{operator} cannot be traced"):
+            torch.jit.trace(traced, (torch.ones(2, 3, 8), torch.ones(8)))

@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import Any, List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -41,6 +42,16 @@ def _activation(activation: Optional[str], known: Tuple[Optional[str], ...]) -> 
     if activation not in known:
         raise ValueError(f"activation must be one of {known}, got {activation!r}")
     return _ACTIVATIONS[activation]
+
+
+def _no_tangent(what: str, *tensors: Any) -> None:
+    """Refuse what the kernels would pass by: forward-mode derivatives, and a trace, which records the allocations only."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative")
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{what} cannot be traced: a trace does not see the kernels")
 
 
 def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -123,6 +134,7 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1,
         ``q (..., K)``, whose rows start at multiples of 16 bytes, and ``scales (ceil(rows / block_rows), ceil(K / 128))``,
         stored with the row index innermost: what ``scaled_matmul`` takes without a copy.
     """
+    _no_tangent("quantize_blocks", x)
     x = _operand(x, "x")
     _no_gradient("quantize_blocks", x)
     if x.dim() < 1 or (block_rows == BLOCK and x.dim() != 2):
@@ -171,6 +183,7 @@ def scaled_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
     may come from the e4m3 matrix instructions, which cut the products of 8 neighbouring columns (``k // 8``) below ``2^-13`` of
     the largest of the eight: 1e-5 of the result for operands of random signs, more where large products of an eight cancel.
     """
+    _no_tangent("scaled_matmul", a_scales, b_scales, bias)
     a = _operand(a, "a", _E4M3_ONLY)
     device = a.device
     b = _operand(b, "b", _E4M3_ONLY, device)
@@ -297,6 +310,7 @@ def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     Returns:
         ``y`` of ``x``'s shape and type, or ``(y, stats)``.  Differentiable by ``x``, ``gamma`` and ``beta`` (once).
     """
+    _no_tangent("group_norm", x, gamma, beta)
     held = _leaves_of(x, gamma, beta) if torch.is_grad_enabled() else None  # before anything here makes a node of them
     x = _operand(x, "x").contiguous()
     act = _activation(activation, (None, "linear", "relu", "swish"))
@@ -318,6 +332,7 @@ def group_norm_gradients(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor,
     """Gradients of ``group_norm`` for a training step that keeps its own tape: ``(dx, dgamma, dbeta)`` from ``dy``, the
     call's arguments and the ``stats`` that it returned.  ``dx`` has ``x``'s type, ``dgamma`` and ``dbeta`` are fp32.
     """
+    _no_tangent("group_norm_gradients", dy, x, gamma, beta, stats)
     x = _operand(x, "x").contiguous()
     device = x.device
     dy = _operand(dy, "dy", (x.dtype,), device).contiguous()
@@ -371,6 +386,7 @@ def dropout(x: torch.Tensor, rate: float, seed: Any, offset: int = 0) -> torch.T
             captured graph that advances it draws a new mask at each replay.
         offset: 64-bit integer, a stream of its own under the same seed (one per call and layer).
     """
+    _no_tangent("dropout", x)
     held = _leaves_of(x) if torch.is_grad_enabled() else None  # before anything here makes a node of it
     x = _operand(x, "x").contiguous()
     rate = float(rate)
