@@ -17,6 +17,19 @@ from ..utils import head_utils
 from .faster_rcnn import Layer
 
 
+def _assigned(held: Optional[torch.Tensor], value: torch.Tensor) -> torch.Tensor:
+    """``value`` written into the tensor that a layer already holds, where it fits, so that optimisers and captured graphs built
+    on that tensor go on with it; ``value`` itself otherwise."""
+    if held is None or held.shape != value.shape or held.dtype != value.dtype or held.device != value.device:
+        return value
+    with torch.no_grad():
+        if value.element_size() == 1:  # 8-bit floating point is copied as bytes
+            held.view(torch.uint8).copy_(value.view(torch.uint8))
+        else:
+            held.copy_(value)
+    return held
+
+
 class QuantizedDense(Layer):
     """A Dense layer whose kernel is stored as e4m3 with a scale per 128 x 128 block, for inference.
 
@@ -42,7 +55,10 @@ class QuantizedDense(Layer):
         return config
 
     def set_weights(self, weights: Sequence[torch.Tensor]) -> None:
-        """``[kernel (inputs, units)]`` or ``[kernel, bias (units,)]``, in the layout of a Keras Dense layer."""
+        """``[kernel (inputs, units)]`` or ``[kernel, bias (units,)]``, in the layout of a Keras Dense layer.
+
+        Weights set again are written into the tensors that the layer has, if they fit: captured graphs then use them.
+        """
         if len(weights) not in (1, 2):
             raise ValueError(f"expected [kernel] or [kernel, bias], got {len(weights)} arrays")
         kernel = torch.as_tensor(weights[0])
@@ -51,12 +67,14 @@ class QuantizedDense(Layer):
         device = kernel.device if kernel.is_cuda else _lib.require_gpu()
         bias = None
         if len(weights) == 2:
-            bias = _lib.device_tensor(weights[1], torch.float32, device).detach().clone()
+            bias = _lib.device_tensor(weights[1], torch.float32, device).detach()
             if tuple(bias.shape) != (self.units,):
                 raise ValueError(f"bias must be ({self.units},), got {tuple(bias.shape)}")
-        rows = kernel.detach().to(device).t().contiguous()
-        self.kernel, self.kernel_scales = head_utils.quantize_blocks(rows, block_rows=head_utils.BLOCK, scale_dtype=self.scale_dtype)
-        self.bias = bias
+        with torch.inference_mode(False):  # tensors made in that mode could not be written again outside it
+            rows = kernel.detach().to(device).t().contiguous()
+            kernel, scales = head_utils.quantize_blocks(rows, block_rows=head_utils.BLOCK, scale_dtype=self.scale_dtype)
+            self.kernel, self.kernel_scales = _assigned(self.kernel, kernel), _assigned(self.kernel_scales, scales)
+            self.bias = None if bias is None else _assigned(self.bias, bias.clone())
 
     def call(self, inputs: torch.Tensor) -> torch.Tensor:
         """``(..., inputs)`` fp32, fp16 or bf16 -> ``(..., units)`` of ``out_dtype``."""
@@ -88,12 +106,15 @@ class GroupNormalization(Layer):
         return config
 
     def set_weights(self, weights: Sequence[torch.Tensor]) -> None:
-        """``[gamma (channels,), beta (channels,)]``."""
+        """``[gamma (channels,), beta (channels,)]``; set again, they are written into the parameters that the layer has, if they
+        fit: optimisers and captured steps built on those go on with them.
+        """
         with torch.inference_mode(False):  # tensors made in that mode could not train later
             gamma, beta = (_lib.device_tensor(w, torch.float32).detach().clone() for w in weights)
             if gamma.dim() != 1 or gamma.shape != beta.shape:
                 raise ValueError(f"gamma and beta must be (channels,), got {tuple(gamma.shape)} and {tuple(beta.shape)}")
-            self.gamma, self.beta = gamma.requires_grad_(self.trainable), beta.requires_grad_(self.trainable)
+            self.gamma = _assigned(self.gamma, gamma).requires_grad_(self.trainable)
+            self.beta = _assigned(self.beta, beta).requires_grad_(self.trainable)
 
     def get_weights(self) -> List[torch.Tensor]:
         return [] if self.gamma is None else [self.gamma, self.beta]
