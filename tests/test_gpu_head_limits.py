@@ -68,3 +68,21 @@ def test_group_norm_by_chunks_of_many_images(head, knobs):
     y, stats = head.group_norm(x[:10], gamma, beta, 2, return_stats=True)
     with pytest.raises(pkg._lib.UnsupportedSizeError, match="threads"):
         head.group_norm_gradients(x, x, gamma, beta, stats[:1].expand(images, 2, 2))
+
+
+def test_dropout_that_keeps_nothing(head):
+    """Where round(rate * 2^32) is 2^32 no word is large enough, not even 2^32 - 1, of which 2^33 elements have a few."""
+    x = torch.ones((1 << 33,), dtype=F16, device="cuda")
+    for seed in (1, 2, 3):
+        y = head.dropout(x, 1 - 2.0 ** -34, seed)
+        assert not y.view(torch.int16).any()
+    del y
+    state = torch.tensor([5, 6], device="cuda")
+    for dtype in (F32, F16, BF16):
+        bad = torch.full((1027,), float("nan"), dtype=dtype, device="cuda")
+        for v in (bad, bad[1:]):
+            for args in ((3,), (state,)):
+                assert (head.dropout(v, 1 - 2.0 ** -53, *args) == 0).all()
+    # words of 2^32 - 1: two in the mean, and a chance of 1e-13 of 20
+    kept = sum(int((part != 0).sum()) for part in head.dropout(x, 1 - 2.0 ** -32, 1).split(1 << 30))
+    assert kept < 20

@@ -80,14 +80,23 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T *__restrict__ x, T
   }
 }
 
+// Where rate * 2^32 rounds to 2^32 no word of 32 bits is large enough: nothing is kept.
 template <typename T>
-static int launch_dropout(const void *x, void *y, long long count, uint32_t threshold, float scale, uint64_t seed,
-                          uint64_t offset, const uint64_t *state, hipStream_t stream) {
+__global__ __launch_bounds__(256) void drop_all_kernel(T *__restrict__ y, long long count) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) y[i] = (T)0.0f;
+}
+
+template <typename T>
+static int launch_dropout(const void *x, void *y, long long count, uint64_t least, float scale, uint64_t seed, uint64_t offset,
+                          const uint64_t *state, hipStream_t stream) {
   const bool aligned = aligned_to(x, 16) && aligned_to(y, 16);
   const int vec = aligned ? (int)(16 / sizeof(T)) : 4;
   long long blocks = ((count + vec - 1) / vec + 255) / 256;
   if (blocks > 16384) blocks = 16384;
-  if (aligned)
+  const uint32_t threshold = (uint32_t)least;
+  if (least >> 32)
+    hipLaunchKernelGGL(drop_all_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream, (T *)y, count);
+  else if (aligned)
     hipLaunchKernelGGL((dropout_kernel<T, 16 / sizeof(T), true>), dim3((unsigned)blocks), dim3(256), 0, stream, (const T *)x,
                        (T *)y, count, threshold, scale, seed, offset, state);
   else
@@ -109,11 +118,10 @@ extern "C" int frcnn_dropout(const void *x, void *y, int type, int64_t count, do
   FRCNN_REQUIRE(x && y, "dropout: null pointer");
   FRCNN_REQUIRE(aligned_to(x, type_bytes(type)) && aligned_to(y, type_bytes(type)), "dropout: pointers must be element aligned");
   FRCNN_REQUIRE(!state || aligned_to(state, 8), "dropout: state must be 8-byte aligned");
-  const double t = rate * 4294967296.0;
-  const uint32_t threshold = t >= 4294967295.0 ? 0xFFFFFFFFu : (uint32_t)__builtin_rint(t);
+  const uint64_t least = (uint64_t)__builtin_rint(rate * 4294967296.0);  // 0 .. 2^32
   const float scale = (float)(1.0 / (1.0 - rate));
   hipStream_t s = (hipStream_t)stream;
-  if (type == FRCNN_F32) return launch_dropout<float>(x, y, count, threshold, scale, seed, offset, state, s);
-  if (type == FRCNN_F16) return launch_dropout<_Float16>(x, y, count, threshold, scale, seed, offset, state, s);
-  return launch_dropout<__bf16>(x, y, count, threshold, scale, seed, offset, state, s);
+  if (type == FRCNN_F32) return launch_dropout<float>(x, y, count, least, scale, seed, offset, state, s);
+  if (type == FRCNN_F16) return launch_dropout<_Float16>(x, y, count, least, scale, seed, offset, state, s);
+  return launch_dropout<__bf16>(x, y, count, least, scale, seed, offset, state, s);
 }
