@@ -86,3 +86,19 @@ def test_dropout_that_keeps_nothing(head):
     # words of 2^32 - 1: two in the mean, and a chance of 1e-13 of 20
     kept = sum(int((part != 0).sum()) for part in head.dropout(x, 1 - 2.0 ** -32, 1).split(1 << 30))
     assert kept < 20
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape,groups", [((2, 4, 1024), 1), ((3, 50, 64), 8)])
+def test_gradients_of_a_dy_between_16_bytes(head, shape, groups, dtype):
+    """A contiguous dy at any element's address gives the bits of an aligned one, with groups of more than 512 channels too."""
+    x = torch.randn(shape, device="cuda").to(dtype)
+    dy = torch.empty(x.numel() + 1, dtype=dtype, device="cuda")[1:].view(shape).normal_()
+    gamma, beta = torch.randn(shape[-1], device="cuda"), torch.randn(shape[-1], device="cuda")
+    _, stats = head.group_norm(x, gamma, beta, groups, activation="swish", return_stats=True)
+    want = head.group_norm_gradients(dy.clone(), x, gamma, beta, stats, activation="swish")
+    for got, exp in zip(head.group_norm_gradients(dy, x, gamma, beta, stats, activation="swish"), want):
+        assert torch.equal(got, exp)
+    leaf = x.clone().requires_grad_()
+    head.group_norm(leaf, gamma, beta, groups, activation="swish").backward(dy)
+    assert torch.equal(leaf.grad, want[0])
