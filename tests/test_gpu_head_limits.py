@@ -102,3 +102,10 @@ def test_gradients_of_a_dy_between_16_bytes(head, shape, groups, dtype):
     leaf = x.clone().requires_grad_()
     head.group_norm(leaf, gamma, beta, groups, activation="swish").backward(dy)
     assert torch.equal(leaf.grad, want[0])
+
+
+@pytest.mark.parametrize("groups", [2.5, 0.5, 0, -2, 3, 20])
+def test_groups_that_do_not_divide(head, groups):
+    """Also fractions that divide: 10 channels are no 2.5 groups."""
+    with pytest.raises(ValueError, match="multiple"):
+        head.group_norm(torch.ones((2, 3, 10), device="cuda"), torch.ones(10, device="cuda"), torch.ones(10, device="cuda"), groups)

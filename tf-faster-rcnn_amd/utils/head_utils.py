@@ -226,7 +226,7 @@ def _norm_shape(x: torch.Tensor, groups: int) -> Tuple[int, int, int]:
     if x.dim() < 2:
         raise ValueError(f"x must be (batch, ..., channels), got {tuple(x.shape)}")
     batch, channels, positions = x.shape[0], x.shape[-1], x.shape[1:-1].numel()
-    if groups < 1 or channels < 1 or channels % groups:
+    if groups < 1 or channels < 1 or channels % groups or groups != int(groups):
         raise ValueError(f"{channels} channels are not a multiple of {groups} groups")
     if positions < 1:
         raise ValueError(f"x needs at least one position per image, got {tuple(x.shape)}")
