@@ -206,74 +206,44 @@ __device__ __forceinline__ void with_output_type(const ProductArgs &p, F f) {
   else f((__bf16 *)nullptr);
 }
 
-// TM x TN tiles of 16 x 16 per workgroup; its W waves share the blocks of K and add their sums in LDS, in the waves' order.  For
-// few rows, where the weights' way from memory is all there is: 116 MB for one row in 24 us, 4.8 TB/s.  More blocks in flight per
-// wave (two, four) gave nothing.
-template <int TM, int TN, int W, int MODE>
-__global__ __launch_bounds__(64 * W) void product_split_kernel(ProductArgs p, int tiles_n) {
+// One 16 x 16 tile per workgroup; its 16 waves share the blocks of K and add their sums in LDS, in the waves' order.  For few
+// rows, where the weights' way from memory is all there is: 116 MB for one row in 24 us, 4.8 TB/s.  More blocks in flight per wave
+// (two, four) gave nothing.
+static const int kSplitWaves = 16;
+
+template <int MODE>
+__global__ __launch_bounds__(64 * kSplitWaves) void product_split_kernel(ProductArgs p, int tiles_n) {
   using S = Scale<MODE>;
   using O = Operand<MODE>;
   const int tn = (int)(blockIdx.x % (unsigned)tiles_n), tm = (int)(blockIdx.x / (unsigned)tiles_n);
   const int wave = threadIdx.x >> 6, lane = lane_id();
-  const int m0 = tm * TM * 16, n0 = tn * TN * 16;
-  const uint8_t *arow[TM], *brow[TN];
-  long long sa_at[TM], sb_at[TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = min(m0 + i * 16 + (lane & 15), p.M - 1);  // rows beyond the end repeat the last one and are not stored
-    arow[i] = p.a + m * p.lda;
-    sa_at[i] = m * p.sa_row;
+  // rows beyond the end repeat the last one and are not stored
+  const int row = min(tm * 16 + (lane & 15), p.M - 1), column = min(tn * 16 + (lane & 15), p.N - 1);
+  const uint8_t *arow = p.a + row * p.lda, *brow = p.b + column * p.ldb;
+  const long long sa_at = row * p.sa_row, sb_at = (long long)(tn * 16 / kQuantBlock) * p.sb_row;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int kb = wave; kb < p.blocks; kb += kSplitWaves) {
+    const typename O::type b = O::of(load_operand(brow, kb, p.K));
+    const float sb = S::load(p.sb, sb_at + kb * p.sb_block);
+    const typename O::type a = O::of(load_operand(arow, kb, p.K));
+    const float sa = S::load(p.sa, sa_at + kb * p.sa_block);
+    const f32x4 d = block_product<MODE>(b, a, f32x4{0, 0, 0, 0}, sb, sa);
+    const float both = sb * sa;
+    if (__builtin_expect(__any(__builtin_amdgcn_classf(both, 0x2F7)), 0) && far_scales(sb, sa))  // no normal number
+      add_far_scaled(acc, d, sb, sa);
+    else
+      add_scaled(acc, d, both);
   }
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int n = min(n0 + j * 16 + (lane & 15), p.N - 1);
-    brow[j] = p.b + n * p.ldb;
-    sb_at[j] = (long long)(min(n0 + j * 16, p.N - 1) / kQuantBlock) * p.sb_row;
-  }
-  f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  for (int kb = wave; kb < p.blocks; kb += W) {
-    typename O::type a[TM], b[TN];
-    typename S::type sa[TM], sb[TN];
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      b[j] = O::of(load_operand(brow[j], kb, p.K));
-      sb[j] = S::load(p.sb, sb_at[j] + kb * p.sb_block);
-    }
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      a[i] = O::of(load_operand(arow[i], kb, p.K));
-      sa[i] = S::load(p.sa, sa_at[i] + kb * p.sa_block);
-    }
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const f32x4 d = block_product<MODE>(b[j], a[i], f32x4{0, 0, 0, 0}, sb[j], sa[i]);
-        const float both = sb[j] * sa[i];
-        if (__builtin_expect(__any(__builtin_amdgcn_classf(both, 0x2F7)), 0) && far_scales(sb[j], sa[i]))  // no normal number
-          add_far_scaled(acc[i][j], d, sb[j], sa[i]);
-        else
-          add_scaled(acc[i][j], d, both);
-      }
-  }
-  __shared__ f32x4 part[W][TM * TN][64];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) part[wave][i * TN + j][lane] = acc[i][j];
+  __shared__ f32x4 part[kSplitWaves][64];
+  part[wave][lane] = acc;
   __syncthreads();
-  for (int t = wave; t < TM * TN; t += W) {
-    f32x4 v = part[0][t][lane];
+  if (wave) return;
+  f32x4 v = part[0][lane];
 #pragma unroll
-    for (int w = 1; w < W; ++w) v += part[w][t][lane];
-    const int m = m0 + (t / TN) * 16 + (lane & 15), n = n0 + (t % TN) * 16 + (lane >> 4) * 4;
-    v += bias4(p, n);
-    if (m < p.M && n < p.N) with_output_type(p, [&](auto *type) { store4<__remove_pointer(decltype(type))>(p, m, n, v); });
-  }
+  for (int w = 1; w < kSplitWaves; ++w) v += part[w][lane];
+  const int m = tm * 16 + (lane & 15), n = tn * 16 + (lane >> 4) * 4;
+  v += bias4(p, n);
+  if (m < p.M && n < p.N) with_output_type(p, [&](auto *type) { store4<__remove_pointer(decltype(type))>(p, m, n, v); });
 }
 
 // ---- large products: tiles through LDS ------------------------------------------------------------------------------------------
@@ -730,18 +700,18 @@ static int launch_tiles(const ProductArgs &p, void *workspace, size_t workspace_
   return launch_tile<2, 2, 2, 4, 2, 3, MODE>(p, f, workspace, workspace_bytes, s);
 }
 
-template <int TM, int TN, int W, int MODE>
+template <int MODE>
 static int launch_split(const ProductArgs &p, hipStream_t s) {
-  const long long tn = ((long long)p.N + TN * 16 - 1) / (TN * 16);
-  const long long most = kGridThreads / (64 * W) / tn * (TM * 16);  // rows of one launch; N <= 2^24 leaves some
+  const long long tn = ((long long)p.N + 15) / 16;
+  const long long most = kGridThreads / (64 * kSplitWaves) / tn * 16;  // rows of one launch; N <= 2^24 leaves some
   for (long long first = 0; first < p.M; first += most) {
     ProductArgs part = p;
     part.M = (int)(p.M - first < most ? p.M - first : most);
     part.a += first * p.lda;
-    part.sa = (const uint8_t *)p.sa + first * p.sa_row * (MODE == kNarrowE8M0 || MODE == kWideE8M0 ? 1 : 4);
+    part.sa = (const uint8_t *)p.sa + first * p.sa_row * (MODE == kWideE8M0 ? 1 : 4);
     part.y = (uint8_t *)p.y + first * p.ldy * (long long)type_bytes(p.out);
-    const long long tm = ((long long)part.M + TM * 16 - 1) / (TM * 16);
-    hipLaunchKernelGGL((product_split_kernel<TM, TN, W, MODE>), dim3((unsigned)(tm * tn)), dim3(64 * W), 0, s, part, (int)tn);
+    const long long tm = ((long long)part.M + 15) / 16;
+    hipLaunchKernelGGL((product_split_kernel<MODE>), dim3((unsigned)(tm * tn)), dim3(64 * kSplitWaves), 0, s, part, (int)tn);
     const int rc = check_launch("scaled_matmul");
     if (rc) return rc;
   }
@@ -751,7 +721,7 @@ static int launch_split(const ProductArgs &p, hipStream_t s) {
 template <int MODE>
 static int launch_product(const ProductArgs &p, void *workspace, size_t workspace_bytes, hipStream_t s) {
   if (use_tiles(p.M, p.N, p.blocks, MODE == kWideF32 || MODE == kWideE8M0)) return launch_tiles<MODE>(p, workspace, workspace_bytes, s);
-  return launch_split<1, 1, 16, MODE == kNarrowE8M0 || MODE == kWideE8M0 ? kWideE8M0 : kWideF32>(p, s);
+  return launch_split<MODE == kNarrowE8M0 || MODE == kWideE8M0 ? kWideE8M0 : kWideF32>(p, s);
 }
 
 }  // namespace frcnn
