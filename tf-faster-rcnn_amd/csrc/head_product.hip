@@ -598,6 +598,11 @@ __global__ __launch_bounds__(64 * WM * WN) void product_join_kernel(ProductArgs 
 // 16640, fp32 scales; `wide`: for fp32 results).  Large tiles move the fewest bytes per product: per product the 160 x 256 tile
 // takes 1.04 times as long as the 256 x 256 one, 128 x 128 1.28 and 64 x 128 1.95 times.  Small ones fill the chip when there are
 // few rows, and waste less of a ragged edge.  `best_form` takes the form with the shortest time by these figures.
+// They are too low for plans cut along K, whose weights come from memory on first touch: 300 rows of 4096 x 28224 are 47 us by them
+// and 63 measured.  The choice was therefore compared with every form forced, 17 to 4800 rows, N = 4096, bf16 results, chosen /
+// best other (us): K = 28224: 64 rows 35 / 39, 150 rows 48 / 52, 300 rows 63 / 69, 600 rows 97 / 104, 1200 rows 163 / 155 (the worst),
+// 2400 rows 280 / 314, 4800 rows 465 / 521; K = 4096: 300 rows 21 / 24, 600 rows 30 / 26 and 1200 rows 39 / 36 (the worst), 2400 rows
+// 43 / 55, 4800 rows 87 / 93.
 struct TileForm {
   int bm, bn, per_cu;
   float block_us, wide_us;

@@ -192,8 +192,9 @@ def case_product(name, rows, units, inner, scales, out, iters):
             "TFLOPs": round(2 * rows * units * inner / ms / 1e9, 1)}
 
 
-def case_quantize(name, rows, inner, dtype, iters):
-    ms = timeit(rotate(lambda i: (torch.randn((rows, inner), device="cuda").to(dtype),), pkg.head_utils.quantize_blocks), iters)
+def case_quantize(name, rows, inner, dtype, iters, block_rows=1):
+    call = lambda x: pkg.head_utils.quantize_blocks(x, block_rows)  # noqa: E731
+    ms = timeit(rotate(lambda i: (torch.randn((rows, inner), device="cuda").to(dtype),), call), iters)
     return {"case": name, "ms": ms, "bytes": rows * inner * (torch.finfo(dtype).bits // 8 + 1)}
 
 
@@ -208,8 +209,10 @@ def case_norm(name, shape, dtype, activation, grad, iters):
     return {"case": name, "ms": ms, "bytes": (5 if grad else 2) * int(np.prod(shape)) * torch.finfo(dtype).bits // 8}
 
 
-def case_dropout(name, shape, dtype, iters):
-    ms = timeit(rotate(lambda i: (torch.randn(shape, device="cuda").to(dtype),), lambda x: pkg.head_utils.dropout(x, 0.5, 1)), iters)
+def case_dropout(name, shape, dtype, iters, layer=False):
+    drop = pkg.box_head.Dropout(0.5, seed=1)
+    call = (lambda x: drop(x, training=True)) if layer else (lambda x: pkg.head_utils.dropout(x, 0.5, 1))
+    ms = timeit(rotate(lambda i: (torch.randn(shape, device="cuda").to(dtype),), call), iters)
     return {"case": name, "ms": ms, "bytes": 2 * int(np.prod(shape)) * torch.finfo(dtype).bits // 8}
 
 
@@ -243,6 +246,14 @@ CASES = {
     "head_norm_pooled_train": lambda it: case_norm("head_norm_pooled_train", (6000, 7, 7, 512), BF16, "swish", True, it),
     "head_norm_maps_train": lambda it: case_norm("head_norm_maps_train", (8, 63, 63, 512), F16, "swish", True, it),
     "head_dropout": lambda it: case_dropout("head_dropout", (6000, 4096), F32, it),
+    "head_fc1_batch_f32": lambda it: case_product("head_fc1_batch_f32", 4800, 4096, 28224, F32, F32, it),
+    "head_quantize_bf16": lambda it: case_quantize("head_quantize_bf16", 4800, 28224, BF16, it),
+    "head_quantize_weights": lambda it: case_quantize("head_quantize_weights", 4096, 28224, F32, it, 128),
+    "head_norm_32_train": lambda it: case_norm("head_norm_32_train", (16, 32, 32, 576), F32, "relu", True, it),
+    "head_norm_31_train": lambda it: case_norm("head_norm_31_train", (16, 31, 31, 512), BF16, "relu", True, it),
+    "head_dropout_bf16": lambda it: case_dropout("head_dropout_bf16", (6000, 4096), BF16, it),
+    "head_dropout_image": lambda it: case_dropout("head_dropout_image", (300, 4096), BF16, it),
+    "head_dropout_layer": lambda it: case_dropout("head_dropout_layer", (300, 4096), BF16, it, layer=True),
 }
 
 
