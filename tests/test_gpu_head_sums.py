@@ -240,3 +240,18 @@ def test_scales_that_are_no_numbers(head, knobs, out_dtype, form):
     want[8, 128:256] = float("nan")
     want = want.to(out_dtype).float()
     assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.nan_to_num(y, nan=1.0), torch.nan_to_num(want, nan=1.0))
+
+
+@pytest.mark.parametrize("form", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+def test_e8m0_scales_at_their_ends(head, knobs, out_dtype, form):
+    """2^127 twice and 2^-127 twice: zeros stay zeros, the smallest sum leaves the range, the largest vanishes, 1 is beside them."""
+    knobs.setenv("FRCNN_PRODUCT_FORM", form)
+    a, b = torch.ones((40, 384), device="cuda"), torch.ones((130, 384), device="cuda")
+    a[:, 128:256], b[:, 128:256] = 448.0, 448.0
+    a[1::2, 256:] = 0.0
+    b[:, 256:], b[:, 256] = 0.0, 2.0 ** -9
+    sa = torch.tensor([127, 0, 254], dtype=torch.uint8, device="cuda").expand(40, 3).contiguous().view(E8M0)
+    sb = torch.tensor([127, 0, 254], dtype=torch.uint8, device="cuda").expand(2, 3).contiguous().view(E8M0)
+    y = head.scaled_matmul(a.to(E4M3), sa, b.to(E4M3), sb, out_dtype=out_dtype)
+    assert (y[1::2] == 128).all() and (y[::2] == float("inf")).all()
